@@ -13,12 +13,18 @@ from .module import (
     Dense,
     Dropout,
     EvalContext,
+    GatedFeedForward,
     Initializer,
+    KeyValueCache,
     LSTMCell,
     MaxBlurPool2D,
     MaxPool2D,
     Module,
+    RMSNorm,
+    SelfAttention,
+    TransformerBlock,
 )
+from .operators import rotary_frequencies
 from .optimizer import Adam, StochasticGradientDescent, add_weight_decay_to_grad
 from .shape import Shape, View
 
@@ -26,5 +32,6 @@ __all__ = [
     "Array", "DualArray", "Parameter", "Scope", "Environment", "Graph",
     "softmax_cross_entropy_accuracy", "softmax_cross_entropy_loss",
     "Conv2D", "Dense", "Dropout", "EvalContext", "Initializer", "LSTMCell", "MaxBlurPool2D", "MaxPool2D", "Module",
+    "RMSNorm", "GatedFeedForward", "SelfAttention", "KeyValueCache", "TransformerBlock", "rotary_frequencies",
     "Adam", "StochasticGradientDescent", "add_weight_decay_to_grad", "Shape", "View",
 ]

@@ -7,6 +7,7 @@ from typing import List, Sequence
 
 from . import kernel as K
 from .graph import Graph
+from .operators import OPERATORS, OperatorKernel
 from .shape import BROADCAST, Shape, View
 
 MAX_DIM = 7
@@ -15,6 +16,7 @@ MAX_DIM = 7
 STATUS_NAMES = ("ok", "invalid", "out of memory", "hip", "compile", "unsupported", "no device")
 
 KIND_FILL, KIND_PER_ELEMENT, KIND_REDUCE, KIND_MATMUL, KIND_UNPAD, KIND_W2I, KIND_SCATTER_ADD = range(7)
+KIND_FIRST_OPERATOR = 7  # DSC_KERNEL_RMS_NORM; operators.OPERATORS lists the kinds from there on
 (PE_LOAD, PE_LITERAL_F32, PE_LITERAL_U32, PE_COORD, PE_RAND, PE_UNARY, PE_BINARY, PE_SELECT, PE_GATHER) = range(9)
 
 SCHEDULE_NO_FUSION = 1
@@ -69,6 +71,8 @@ class CKernelDesc(C.Structure):
         ("stride_w", C.c_int32),
         ("stride_h", C.c_int32),
         ("output_mode", C.c_int32),
+        ("op_int", C.c_int32 * 4),
+        ("op_float", C.c_uint32 * 2),
     ]
 
 
@@ -225,6 +229,18 @@ class MarshalledKernel:
             d.shape = c_shape(kernel.shape)
             views = (kernel.values, kernel.indices)
             d.axis = kernel.axis
+        elif isinstance(kernel, OperatorKernel):
+            spec = kernel.spec
+            d.kind = KIND_FIRST_OPERATOR + OPERATORS.index(spec.name)
+            d.shape = c_shape(kernel.shape)
+            views = kernel.inputs
+            outs = (C.c_int32 * len(kernel.results))(*kernel.results)
+            d.n_outputs, d.outputs = len(kernel.results), outs
+            for i, value in enumerate(spec.ints):
+                d.op_int[i] = value
+            for i, value in enumerate(spec.floats):
+                d.op_float[i] = K.f32_bits(value)
+            self._keep.append(outs)
         else:
             raise TypeError(f"unknown kernel {kernel!r}")
         arr = _view_array(views)

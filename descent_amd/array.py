@@ -18,6 +18,20 @@ import numpy as np
 
 from .graph import Graph, MOV, Op, OpGraph
 from .kernel import Literal
+from .operators import (
+    ACTIVATIONS,
+    DUAL_BOTH,
+    DUAL_GATED,
+    DUAL_SUM,
+    OperatorSpec,
+    attention_ints,
+    attention_splits,
+    dual_matmul_shapes,
+    emit,
+    norm_partials,
+    norm_spec,
+    rotary_spec,
+)
 from .shape import BATCHES, ROWS, Shape, View
 
 
@@ -379,6 +393,71 @@ class Array:
         shape = self.shape.windows_to_image(stride_wh)
         return Array(s.ops.new_node(s.colour, shape, Op("WindowsToImage", tuple(stride_wh)), [self.node_id]), s)
 
+    # -- sequence-model operators (kernels of their own; see operators.py) ---------------
+    def _rows(self) -> "Array":
+        n = self.shape[-1]
+        return self.reshape([self.shape.element_count() // n, n])
+
+    def _rms_norm(self, weight: "Array", epsilon: float, residual, count: int) -> List["Array"]:
+        spec = norm_spec(self.shape, weight.shape, epsilon, None if residual is None else residual.shape)
+        operands = [self._rows(), weight] + ([] if residual is None else [residual._rows()])
+        return emit(operands, spec, count)
+
+    def rms_norm(self, weight, epsilon: float = 1e-6) -> "Array":
+        """self / sqrt(mean(self^2) + epsilon) * weight over the last axis; weight is [n]."""
+        return self._rms_norm(self._lift(weight), epsilon, None, 1)[0].reshape(self.shape)
+
+    def add_rms_norm(self, residual, weight, epsilon: float = 1e-6) -> Tuple["Array", "Array"]:
+        """(rms_norm(sum), sum) with sum = self + residual, in one pass."""
+        y, total = self._rms_norm(self._lift(weight), epsilon, self._lift(residual), 2)
+        return y.reshape(self.shape), total.reshape(self.shape)
+
+    def rotary(self, frequencies, positions=None, layout: str = "half", magnitude: float = 1.0, inverse: bool = False) -> "Array":
+        """Rotary positions on [batch, tokens, heads, dim]: pair i of a head is turned by position * frequencies[i]
+        (`rotary_frequencies` makes tables) and scaled by `magnitude`; elements past the pairs pass through.
+
+        layout     "half": pair i is (i, i + pairs); "interleaved": (2 i, 2 i + 1)
+        positions  u32 array: [batch], the position of each sequence's first token (the others follow), or
+                   [batch, tokens]; None counts from 0
+        inverse    turns back (the gradient of the rotation, with the same magnitude)"""
+        frequencies = self._lift(frequencies)
+        positions = None if positions is None else self._lift(positions)
+        spec = rotary_spec(self.shape, frequencies.shape, None if positions is None else positions.shape, layout, magnitude, inverse)
+        return emit([self, frequencies] + ([] if positions is None else [positions]), spec, 1)[0]
+
+    def _attention(self, k, v, window, sinks, scale, start, length):
+        """(output, log of the softmax's denominator per query and head, integer attributes, scale)"""
+        scale = float(self.shape[-1]) ** -0.5 if scale is None else float(scale)
+        if not abs(scale) < float("inf"):
+            raise ValueError(f"attention: scale must be finite, got {scale}")
+        ints = attention_ints(self.shape, k.shape, v.shape, window, sinks, *(None if a is None else a.shape for a in (start, length)))
+        splits = attention_splits(self.shape, k.shape, window, sinks)
+        operands = [self, k, v] + [a for a in (start, length) if a is not None]
+        out, lse = emit(operands, OperatorSpec("Attention", ints + (splits,), (scale,)), 2)
+        if splits > 1:
+            out, lse = emit([out, lse], OperatorSpec("AttentionJoin"), 2)
+        return out, lse, ints, scale
+
+    def attention(self, k, v, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None, start=None,
+                  length=None) -> "Array":
+        """softmax(scale q k^T) v for queries [batch, tokens, heads, dim] and keys and values [batch, keys, groups, dim];
+        heads h * heads / groups .. share key head h.
+
+        Token t of sequence b stands at position start[b] + t and sees key j when j <= position, j < length[b] and,
+        with a window, j > position - window or j < sinks.  A token at or past length[b] is padding: it sees nothing,
+        and a token that sees nothing gets zeros.  `start` and `length` are u32 arrays [batch]; without them the
+        queries are the last tokens of the keys, and every key counts.  `scale` defaults to dim^-0.5."""
+        k, v = self._lift(k), self._lift(v)
+        start, length = (None if a is None else self._lift(a) for a in (start, length))
+        return self._attention(k, v, window, sinks, scale, start, length)[0]
+
+    def gated_dense(self, w_gate, w_up, activation: str = "silu") -> "Array":
+        """activation(self w_gate) * (self w_up) for [rows, width] and two [width, hidden] weights: both products, the
+        activation ("silu", "gelu", "relu" or "sigmoid") and the product of the two in one kernel."""
+        w_gate, w_up = self._lift(w_gate), self._lift(w_up)
+        dual_matmul_shapes(self.shape, w_gate.shape, w_up.shape, activation)
+        return emit([self, w_gate, w_up], OperatorSpec("DualMatMul", (DUAL_GATED, ACTIVATIONS.index(activation))), 1)[0]
+
 
 class DualArray:
     """(value, d loss / d value) pair (src/array.rs:20-25, 794-1147)."""
@@ -631,6 +710,72 @@ class DualArray:
         return (
             windows.reshape([m * oh * ow * g, fh * fw, nc]).reduce_max(1, True).reshape([m, oh, ow, g * nc])
         )
+
+    # -- sequence-model operators (see Array's methods of the same names) ----------------
+    def _rms_norm(self, weight, epsilon: float, residual):
+        x, dx = self.into_inner()
+        w, dw = self._lift(weight).into_inner()
+        r, dr = (None, None) if residual is None else self._lift(residual).into_inner()
+        y, total, inverse_rms = x._rms_norm(w, epsilon, r, 3)
+        if r is None:
+            total = x._rows()
+        y, dy = y.reshape(x.shape).with_empty_grad()
+        operands = [total, inverse_rms, w, dy._rows()]
+        if r is not None:
+            total, dtotal = total.reshape(x.shape).with_empty_grad()
+            operands.append(dtotal._rows())
+        rows = inverse_rms.shape[0]
+        ds, partial = emit(operands, OperatorSpec("RmsNormGrad", (int(r is not None), norm_partials(rows))), 2)
+        ds = ds.reshape(x.shape)
+        dx.accumulate(ds)
+        if r is not None:
+            dr.accumulate(ds)
+        dw.accumulate(partial.reduce_sum(0, False) if len(partial.shape) == 2 and partial.shape[0] > 1 else partial.reshape(w.shape))
+        return DualArray(y, dy), None if r is None else DualArray(total, dtotal)
+
+    def rms_norm(self, weight, epsilon: float = 1e-6):
+        return self._rms_norm(weight, epsilon, None)[0]
+
+    def add_rms_norm(self, residual, weight, epsilon: float = 1e-6):
+        """(norm, sum): the gradients that arrive at both leave in one pass, and a sum that nothing reads costs nothing."""
+        return self._rms_norm(weight, epsilon, residual)
+
+    def rotary(self, frequencies, positions=None, layout: str = "half", magnitude: float = 1.0):
+        """Frequencies and positions are plain arrays and get no gradient."""
+        a, da = self.into_inner()
+        b, db = a.rotary(frequencies, positions, layout, magnitude).with_empty_grad()
+        da.accumulate(db.rotary(frequencies, positions, layout, magnitude, inverse=True))
+        return DualArray(b, db)
+
+    def attention(self, k, v, window: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None, start=None, length=None):
+        q, dq = self.into_inner()
+        k, dk = self._lift(k).into_inner()
+        v, dv = self._lift(v).into_inner()
+        start, length = (None if a is None else q._lift(a) for a in (start, length))
+        out, lse, ints, scale = q._attention(k, v, window, sinks, scale, start, length)
+        out, dout = out.with_empty_grad()
+        places = [a for a in (start, length) if a is not None]
+        grad_q, delta = emit([q, k, v, out, dout, lse] + places, OperatorSpec("AttentionGradQuery", ints, (scale,)), 2)
+        grad_k, grad_v = emit([q, k, v, dout, lse, delta] + places, OperatorSpec("AttentionGradKeyValue", ints, (scale,)), 2)
+        dq.accumulate(grad_q)
+        dk.accumulate(grad_k)
+        dv.accumulate(grad_v)
+        return DualArray(out, dout)
+
+    def gated_dense(self, w_gate, w_up, activation: str = "silu"):
+        x, dx = self.into_inner()
+        wg, dwg = self._lift(w_gate).into_inner()
+        wu, dwu = self._lift(w_up).into_inner()
+        dual_matmul_shapes(x.shape, wg.shape, wu.shape, activation)
+        act = ACTIVATIONS.index(activation)
+        h, gate, up = emit([x, wg, wu], OperatorSpec("DualMatMul", (DUAL_GATED, act)), 3)
+        h, dh = h.with_empty_grad()
+        dgate, dup = emit([gate, up, dh], OperatorSpec("GatedGrad", (act,)), 2)
+        dx.accumulate(emit([dgate, dup, wg.transpose(), wu.transpose()], OperatorSpec("DualMatMul", (DUAL_SUM, 0)), 1)[0])
+        grad_gate, grad_up = emit([x.transpose(), dgate, dup], OperatorSpec("DualMatMul", (DUAL_BOTH, 0)), 2)
+        dwg.accumulate(grad_gate)
+        dwu.accumulate(grad_up)
+        return DualArray(h, dh)
 
     def set_loss(self) -> Array:
         self.loss_grad()._set_loss_grad_root()

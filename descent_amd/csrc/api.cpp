@@ -498,6 +498,7 @@ int dsc_kernel_launch(dsc_ctx* ctx, dsc_kernel* kernel, const dsc_buf* bufs, int
         if (!ctx->c.heap.info(bufs[i], &ptrs[i], &size)) return fail(DSC_ERR_INVALID, "unknown buffer handle in launch");
         size_t need = 0;
         if (i < d.n_inputs) need = (size_t)element_count(d.inputs[i].in_shape) * 4;
+        else if (is_operator(d.kind)) need = (size_t)element_count(operator_results(d)[d.outputs[i - d.n_inputs]]) * 4;
         else need = (size_t)element_count(d.shape) * 4;
         if (size < need) return fail(DSC_ERR_INVALID, "buffer " + std::to_string(i) + " of '" + k->label + "' is too small");
     }

@@ -13,8 +13,12 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libdescent_hip.so")
-SOURCES = ["desc.cpp", "codegen.cpp", "runtime.cpp", "schedule.cpp", "api.cpp"]
-EMBED = {"kPreludeSource": "kernels/prelude.inc", "kMatmulMfmaSource": "kernels/matmul_mfma.inc"}
+SOURCES = ["desc.cpp", "codegen.cpp", "operators.cpp", "runtime.cpp", "schedule.cpp", "api.cpp"]
+EMBED = {
+    "kPreludeSource": "kernels/prelude.inc", "kMatmulMfmaSource": "kernels/matmul_mfma.inc",
+    "kRmsNormSource": "kernels/rms_norm.inc", "kRotarySource": "kernels/rotary.inc",
+    "kAttentionSource": "kernels/attention.inc", "kDualMatmulSource": "kernels/dual_matmul.inc",
+}
 
 
 def embed() -> str:

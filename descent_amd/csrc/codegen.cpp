@@ -4182,7 +4182,7 @@ FusedKernel FusedKernel::plain(const dsc_kernel_desc& d) {
     fk.main = KernelDesc(d);
     const int n_in = fk.main.raw().n_inputs;
     int n_out = 1;
-    if (d.kind == DSC_KERNEL_PER_ELEMENT) n_out = d.n_outputs;
+    if (d.kind == DSC_KERNEL_PER_ELEMENT || is_operator(d.kind)) n_out = d.n_outputs;
     for (int i = 0; i < n_in; ++i) {
         Source s;
         s.buffer = i;
@@ -4324,6 +4324,7 @@ bool can_be_part(const FusedKernel& fk) {
     if (!fk.parts.empty() || fk.binned_stage || fk.chain_group) return false;
     if (fk.dgrad.on && conv_bwd_loader_waves_impl(fk)) return false;  // 512 threads per workgroup
     if (fk.dgrad.on || fk.cfwd.on || !fk.row_stages.empty()) return true;
+    if (is_operator(fk.main.raw().kind)) return false;
     if (fk.main.raw().kind != DSC_KERNEL_MATMUL) return true;
     // of the MatMul kernels, the row-per-thread, short-k and tall-k ones run 256 threads addressed by blockIdx.x
     const MatMulDims g = matmul_dims(fk.main.raw());
@@ -4350,6 +4351,15 @@ std::string generate(const FusedKernel& fk, Generated* out) {
 static std::string generate_one(const FusedKernel& fk, Generated* out, bool with_prelude) {
     string err = validate(fk.main.raw());
     if (!err.empty()) return err;
+    if (is_operator(fk.main.raw().kind)) {
+        if (!fk.virtuals.empty() || fk.has_epilogue || !fk.row_stages.empty()) return "an operator takes no fused producers or consumers";
+        Generated g;
+        err = generate_operator(fk, &g);
+        if (!err.empty()) return err;
+        g.n_buffers = fk.n_buffers;
+        *out = g;
+        return "";
+    }
     for (auto& v : fk.virtuals) {
         err = validate(v.pe.raw());
         if (!err.empty()) return "fused producer: " + err;

@@ -281,11 +281,19 @@ bool dot_kernel_shape(const MatMulDims& g);
 // one layer with a few outputs (see FusedKernel::GradPair; which buffers they read is the caller's to compare)
 bool grad_pair_shapes(const FusedKernel& s, const FusedKernel& t, int64_t* chunk_rows, int64_t* chunks);
 
+// Source of an operator's kernel (operators.cpp); fills everything of `out` but n_buffers.
+std::string generate_operator(const FusedKernel& fk, Generated* out);
+
 // hipRTC options every kernel is compiled with (after --offload-arch=<arch>).
 const std::vector<std::string>& compile_options();
 
 // The prelude and matmul template texts (embedded at build time from kernels/*.inc).
 extern const char* const kPreludeSource;
 extern const char* const kMatmulMfmaSource;
+// the operators' kernels
+extern const char* const kRmsNormSource;
+extern const char* const kRotarySource;
+extern const char* const kAttentionSource;
+extern const char* const kDualMatmulSource;
 
 }  // namespace dsc

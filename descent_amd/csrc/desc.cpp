@@ -67,7 +67,12 @@ std::string KernelDesc::key() const {
     case DSC_KERNEL_WINDOWS_TO_IMAGE: put(s, d.stride_w); put(s, d.stride_h); break;
     case DSC_KERNEL_SCATTER_ADD: put(s, d.axis); break;
     case DSC_KERNEL_MATMUL: put(s, d.output_mode); break;
-    default: break;
+    default:
+        if (is_operator(d.kind)) {
+            put(s, d.op_int);
+            put(s, d.op_float);
+        }
+        break;
     }
     return s;
 }
@@ -81,7 +86,7 @@ int buffer_count(const dsc_kernel_desc& d) {
     case DSC_KERNEL_WINDOWS_TO_IMAGE: return 2;
     case DSC_KERNEL_MATMUL:
     case DSC_KERNEL_SCATTER_ADD: return 3;
-    default: return 0;
+    default: return is_operator(d.kind) ? d.n_inputs + d.n_outputs : 0;
     }
 }
 
@@ -127,7 +132,7 @@ std::string label_name(const dsc_kernel_desc& d) {
     case DSC_KERNEL_UNPAD: return "Unpad " + shape_str(d.shape);
     case DSC_KERNEL_WINDOWS_TO_IMAGE: return "WindowsToImage " + shape_str(d.shape);
     case DSC_KERNEL_SCATTER_ADD: return "ScatterAdd " + shape_str(d.inputs[0].out_shape);
-    default: return "?";
+    default: return is_operator(d.kind) ? operator_label(d) : "?";
     }
 }
 
@@ -263,7 +268,7 @@ std::string validate(const dsc_kernel_desc& d) {
             if (i != d.axis && v.out_shape.dims[i] != d.shape.dims[i]) return "scatter_add: values shape mismatch";
         return "";
     }
-    default: return "unknown kernel kind";
+    default: return is_operator(d.kind) ? validate_operator(d) : "unknown kernel kind";
     }
 }
 

@@ -2264,6 +2264,7 @@ struct Planner {
                 }
                 for (int ci : cons) {
                     Draft& q = drafts[ci];
+                    if (is_operator(q.fk.main.raw().kind)) ok = false;  // operators read buffers
                     if (ci <= i) ok = false;
                     for (auto& o : q.outs)
                         if (o.copy_from == node) ok = false;  // updated in place by the consumer
@@ -3273,7 +3274,8 @@ int Schedule::build(Context* ctx, const dsc_schedule_desc& desc, uint32_t flags)
         std::string err = validate(cl.kernel);
         if (!err.empty()) return fail(DSC_ERR_INVALID, "schedule: cluster " + std::to_string(c) + ": " + err);
         const int want_in = cl.kernel.kind == DSC_KERNEL_FILL ? 0 : cl.kernel.n_inputs;
-        const int want_out = cl.kernel.kind == DSC_KERNEL_PER_ELEMENT ? cl.kernel.n_outputs : 1;
+        const bool lists_outputs = cl.kernel.kind == DSC_KERNEL_PER_ELEMENT || is_operator(cl.kernel.kind);
+        const int want_out = lists_outputs ? cl.kernel.n_outputs : 1;
         if (cl.n_inputs != want_in || cl.n_outputs != want_out)
             return fail(DSC_ERR_INVALID, "schedule: cluster " + std::to_string(c) + " binds the wrong number of nodes");
         Draft& d = drafts[c];

@@ -198,6 +198,8 @@ class Environment:
             raise ValueError("parameter has no initializer")
         if init.kind == "zero":
             self.writer(parameter).zero_fill()
+        elif init.kind == "constant":
+            self.write_parameter(parameter, np.full(n, init.scale, np.float32))
         elif init.kind == "normal":
             self.write_parameter(parameter, (rng.standard_normal(n) * init.scale).astype(np.float32))
         else:
@@ -212,15 +214,24 @@ class Environment:
         f(scope)
         return scope.build_graph()
 
+    def _schedule(self, graph: Graph):
+        key = (id(self.backend), self.fused)
+        cache = graph.__dict__.setdefault("_schedules", {})
+        sched = cache.get(key)
+        if sched is None:
+            sched = cache[key] = self.backend.make_schedule(graph, self.fused)
+        return sched
+
+    def prepare(self, graph: Graph) -> None:
+        """Plans the graph's launches and compiles their kernels now instead of in the first run."""
+        if self.use_schedule:
+            self._schedule(graph)
+
     def run(self, graph: Graph, rand_seed: int) -> None:
         """src/environment.rs:326-516"""
         rand_seed &= 0xFFFFFFFF
         if self.use_schedule:
-            key = (id(self.backend), self.fused)
-            cache = graph.__dict__.setdefault("_schedules", {})
-            sched = cache.get(key)
-            if sched is None:
-                sched = cache[key] = self.backend.make_schedule(graph, self.fused)
+            sched = self._schedule(graph)
             handles = [p.checked(self).buffer for p in sched.params]
             handles = sched.run(handles, rand_seed)
             for p, h in zip(sched.params, handles):
@@ -233,11 +244,7 @@ class Environment:
         and every parameter the graph writes alternates between its buffer and one spare buffer, allocated here the
         first time the parameter is written this way -- after that a step allocates no device memory at all."""
         rand_seed &= 0xFFFFFFFF
-        key = (id(self.backend), self.fused)
-        cache = graph.__dict__.setdefault("_schedules", {})
-        sched = cache.get(key)
-        if sched is None:
-            sched = cache[key] = self.backend.make_schedule(graph, self.fused)
+        sched = self._schedule(graph)
         written = set(sched.written_slots())
         spare = []
         for i, p in enumerate(sched.params):

@@ -31,6 +31,7 @@ from .kernel import (
     UnpadKernel,
     WindowsToImageKernel,
 )
+from .operators import OperatorKernel, OperatorSpec
 from .shape import Shape, View
 
 MAX_OP_ARGS = 4  # src/op.rs:72
@@ -42,7 +43,8 @@ class Op:
     Input/Output(a=parameter), Literal(a=Literal), Coord, Rand(a=uid),
     Unary(a=name), Binary(a=name), Select(a=mode), MatMul(a=output_mode),
     Reduce(a=name, b=axis), Unpad(a=axis, b=pad), WindowsToImage(a=(sw,sh)),
-    Gather(a=axis), ScatterAdd(a=axis)."""
+    Gather(a=axis), ScatterAdd(a=axis).  Beside the reference's: Operator(a=OperatorSpec), a sequence-model operator
+    whose node is its first result, and Result(a=index), a further result of the operator node that is its argument."""
 
     kind: str
     a: object = None
@@ -72,6 +74,8 @@ class Op:
             return f"Reduce{self.a}({self.b})"
         if self.kind == "Literal":
             return repr(self.a)
+        if self.kind == "Operator":
+            return str(self.a)
         return self.kind
 
 
@@ -235,6 +239,7 @@ class Graph:
         self.clusters: Dict[int, Cluster] = {}
         self.clusters_sorted: List[int] = []
 
+        self._drop_absent_gradients()
         self._rebuild_ordering()
         self._eliminate_dead_code()
         self._rebuild_ordering()
@@ -252,6 +257,21 @@ class Graph:
     def _rebuild_ordering(self):
         self.ops_sorted = self.ops.topo_order()
         assert len(self.ops_sorted) == len(self.ops.nodes), "op graph has a cycle"
+
+    def _drop_absent_gradients(self):
+        """A norm's gradient takes the gradient of the sum that the norm left beside its result; where nothing read that
+        sum, the operand goes."""
+        ops = self.ops
+        for nid, node in ops.nodes.items():
+            if node.op.kind != "Operator" or node.op.a.name != "RmsNormGrad" or not node.op.a.ints[0]:
+                continue
+            eid = ops.arg_edge_ids(nid)[4]
+            source = ops.edges[eid].src
+            while ops.nodes[source].op == MOV and ops.in_edges(source):
+                source = ops.edges[ops.in_edges(source)[0]].src
+            if ops.nodes[source].op == MOV:
+                ops.remove_edge(eid)
+                node.op = Op("Operator", OperatorSpec("RmsNormGrad", (0,) + node.op.a.ints[1:]))
 
     def _eliminate_dead_code(self):
         """Keep what reaches an Output (src/graph.rs:150-165)."""
@@ -281,8 +301,9 @@ class Graph:
             can_reshape = ops.nodes[in_node].op.can_reshape()
             out_eids = ops.out_edges(nid)
             ok = all(
-                ops.nodes[ops.edges[e].dst].op.kind != "Output"
+                (ops.nodes[ops.edges[e].dst].op.kind != "Output" or self._is_operators_output(in_edge, out_eids))
                 and in_edge.view.can_view_through(ops.edges[e].view, can_reshape)
+                and self._operator_reads(in_edge, ops.edges[e], can_reshape)
                 for e in out_eids
             )
             if ok:
@@ -291,6 +312,29 @@ class Graph:
                     assert in_edge.arg == 0
                     ops.add_edge(in_node, oe.dst, oe.arg, in_edge.view.through(oe.view, can_reshape))
                 ops.remove_node(nid)
+
+    def _is_operators_output(self, in_edge: OpEdge, out_eids) -> bool:
+        """Whether a Mov in front of an Output only renames an operator's result: the result's own buffer then becomes
+        the parameter's, which it can for one parameter."""
+        ops = self.ops
+        if ops.nodes[in_edge.src].op.kind not in ("Operator", "Result") or not in_edge.view.is_contiguous():
+            return False
+        readers = [ops.edges[e].dst for e in out_eids] + ops.successors(in_edge.src)
+        return sum(ops.nodes[n].op.kind == "Output" for n in readers) == 1
+
+    def _operator_reads(self, in_edge: OpEdge, edge: OpEdge, can_reshape: bool) -> bool:
+        """Whether the node behind `edge`, where it is an operator, reads `in_edge`'s source without the Mov between
+        them: an operator binds buffers (no literals, no built-ins) and reads certain strided views only."""
+        ops = self.ops
+        op = ops.nodes[edge.dst].op
+        if op.kind == "Result":
+            return False
+        if op.kind != "Operator":
+            return True
+        source = ops.nodes[in_edge.src].op
+        if source.kind == "Literal" or source.is_builtin():
+            return False
+        return op.a.reads_in_place(edge.arg, in_edge.view.through(edge.view, can_reshape))
 
     def _simplify_arithmetic(self):
         """x*1, x+0 (and the u32 forms) become Mov (src/graph.rs:221-253)."""
@@ -535,7 +579,17 @@ class Graph:
                     [values.node_id, indices.node_id],
                     [ClusterOutput(nid, copy_from=acc.node_id)],
                 )
-            elif op.kind in ("Input", "Output", "Literal", "Coord", "Rand"):
+            elif op.kind == "Operator":
+                results = {ops.nodes[s].op.a: s for s in ops.successors(nid) if ops.nodes[s].op.kind == "Result"}
+                kept = sorted(results)
+                cluster = Cluster(
+                    OperatorKernel(op.a, tuple(s.view for s in src), (0, *kept)),
+                    [s.node_id for s in src],
+                    [ClusterOutput(nid)] + [ClusterOutput(results[i]) for i in kept],
+                )
+                for i in kept:
+                    ops.nodes[results[i]].cluster_id = next_cluster
+            elif op.kind in ("Input", "Output", "Literal", "Coord", "Rand", "Result"):
                 continue
             else:
                 raise AssertionError(f"per-element op {op} left unclustered")

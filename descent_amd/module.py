@@ -11,19 +11,25 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from .array import DualArray, Parameter
+from .array import Array, DualArray, Parameter
+from .operators import rotary_frequencies
 
 
 @dataclass(frozen=True)
 class Initializer:
     """src/parameter.rs:10-26"""
 
-    kind: str  # "zero" | "normal" | "uniform"
+    kind: str  # "zero" | "constant" | "normal" | "uniform"
     scale: float = 0.0
 
     @staticmethod
     def zero():
         return Initializer("zero")
+
+    @staticmethod
+    def constant(value: float):
+        """Beside the reference's: every element `value` (the weight of a norm starts at 1)."""
+        return Initializer("constant", float(np.float32(value)))
 
     @staticmethod
     def rand_normal(scale: float):
@@ -161,3 +167,134 @@ class LSTMCell(Module):
             prev_hidden = output_gate * cell.tanh()
             prev_cell = cell
         return prev_hidden
+
+
+class RMSNorm(Module):
+    """Root-mean-square norm over the last axis (no counterpart in the reference)."""
+
+    def __init__(self, env, n: int, epsilon: float = 1e-6):
+        self.weight = env.trainable_parameter([n], "weight", Initializer.constant(1.0))
+        self.epsilon = epsilon
+
+    def eval(self, x, ctx):
+        x.scope.next_colour()
+        return x.rms_norm(self.weight, self.epsilon)
+
+    def add(self, x, residual):
+        """(norm of x + residual, x + residual), for arrays with or without gradients."""
+        x.scope.next_colour()
+        return x.add_rms_norm(residual, self.weight, self.epsilon)
+
+
+class GatedFeedForward(Module):
+    """activation(x w_gate) * (x w_up), then w_down, on [rows, n] (no counterpart in the reference)."""
+
+    def __init__(self, env, n: int, n_hidden: int, activation: str = "silu"):
+        scale = Initializer.rand_normal(float(n) ** -0.5)
+        self.w_gate = env.trainable_parameter([n, n_hidden], "w_gate", scale)
+        self.w_up = env.trainable_parameter([n, n_hidden], "w_up", scale)
+        self.w_down = env.trainable_parameter([n_hidden, n], "w_down", Initializer.rand_normal(float(n_hidden) ** -0.5))
+        self.activation = activation
+
+    def eval(self, x, ctx):
+        x.scope.next_colour()
+        return x.gated_dense(self.w_gate, self.w_up, self.activation).matmul(self.w_down)
+
+
+class KeyValueCache:
+    """Rotated keys and values of `batch` sequences of up to `capacity` tokens, as SelfAttention.step keeps them.  A slot is
+    zero until its token is written; `reset` empties the cache for new sequences."""
+
+    def __init__(self, env, batch: int, capacity: int, groups: int, head_dim: int):
+        self.batch, self.capacity, self.groups, self.head_dim = batch, capacity, groups, head_dim
+        self.keys = env.static_parameter([batch * capacity, groups * head_dim], "keys")
+        self.values = env.static_parameter([batch * capacity, groups * head_dim], "values")
+        self.reset(env)
+
+    def reset(self, env) -> None:
+        for p in (self.keys, self.values):
+            env.writer(p).zero_fill()
+
+    def append(self, scope, parameter: Parameter, new: Array, start: Array) -> Array:
+        """Writes new [batch, tokens, groups, dim] behind the `start` tokens that each sequence holds, in place (a
+        ScatterAdd onto zeros), and returns the whole array.  Tokens past the capacity are dropped."""
+        batch, tokens, groups, dim = new.shape
+        if [batch, groups, dim] != [self.batch, self.groups, self.head_dim]:
+            raise ValueError(f"cache holds [{self.batch}, {self.capacity}, {self.groups}, {self.head_dim}], got {new.shape!r}")
+        place = start.reshape([batch, 1]) + scope.coord(tokens).value().into_u32()
+        row = scope.coord(batch).value().into_u32().reshape([batch, 1]) * self.capacity + place
+        # (an index past the array is dropped; this one is, whatever the array)
+        row = place.into_f32().select_gt(float(self.capacity - 1), scope.literal_u32(0x7F000000), row).reshape([batch * tokens])
+        whole = scope.parameter_value(parameter).scatter_add(new.reshape([batch * tokens, groups * dim]), 0, row)
+        scope.write_parameter_value(parameter, whole)
+        return whole.reshape([self.batch, self.capacity, groups, dim])
+
+
+class SelfAttention(Module):
+    """Causal self-attention on [batch, tokens, n] with rotary positions, grouped key heads and, on request, a sliding
+    window with sinks (no counterpart in the reference)."""
+
+    def __init__(self, env, n: int, heads: int, groups=None, head_dim=None, window=None, sinks: int = 0, frequencies=None):
+        self.heads, self.groups = heads, groups or heads
+        self.head_dim = head_dim or n // heads
+        self.window, self.sinks = window, sinks
+        scale = Initializer.rand_normal(float(n) ** -0.5)
+        self.w_query = env.trainable_parameter([n, heads * self.head_dim], "w_query", scale)
+        self.w_key = env.trainable_parameter([n, self.groups * self.head_dim], "w_key", scale)
+        self.w_value = env.trainable_parameter([n, self.groups * self.head_dim], "w_value", scale)
+        self.w_out = env.trainable_parameter([heads * self.head_dim, n], "w_out", Initializer.rand_normal(float(heads * self.head_dim) ** -0.5))
+        table = rotary_frequencies(self.head_dim // 2 * 2) if frequencies is None else np.asarray(frequencies, np.float32)
+        self.frequencies = env.static_parameter_with_data([len(table)], "frequencies", table)
+
+    def _heads(self, x, start):
+        batch, tokens, n = x.shape
+        x.scope.next_colour()
+        rows = x.reshape([batch * tokens, n])
+        q = rows.matmul(self.w_query).reshape([batch, tokens, self.heads, self.head_dim])
+        k = rows.matmul(self.w_key).reshape([batch, tokens, self.groups, self.head_dim])
+        v = rows.matmul(self.w_value).reshape([batch, tokens, self.groups, self.head_dim])
+        return q.rotary(self.frequencies, start), k.rotary(self.frequencies, start), v
+
+    def _out(self, y):
+        batch, tokens, heads, dim = y.shape
+        rows = y.reshape([batch * tokens, heads * dim]).matmul(self.w_out)
+        return rows.reshape([batch, tokens, rows.shape[-1]])
+
+    def eval(self, x, ctx, length=None):
+        """`length`: u32 array [batch] of a padded batch's sequence lengths."""
+        q, k, v = self._heads(x, None)
+        return self._out(q.attention(k, v, self.window, self.sinks, length=length))
+
+    def cache(self, env, batch: int, capacity: int) -> KeyValueCache:
+        return KeyValueCache(env, batch, capacity, self.groups, self.head_dim)
+
+    def step(self, x: Array, cache: KeyValueCache, start: Array) -> Array:
+        """Serving: x [batch, tokens, n] holds the next tokens (usually one) of sequences that have `start` (u32 [batch])
+        tokens in the cache; their keys and values are appended and they attend to all that precede them."""
+        q, k, v = self._heads(x, start)
+        keys = cache.append(x.scope, cache.keys, k, start)
+        values = cache.append(x.scope, cache.values, v, start)
+        return self._out(q.attention(keys, values, self.window, self.sinks, start=start))
+
+
+class TransformerBlock(Module):
+    """x + attention(norm(x)), then the same with the gated feed-forward, on [batch, tokens, n] (no counterpart in the
+    reference)."""
+
+    def __init__(self, env, n: int, heads: int, n_hidden: int, groups=None, head_dim=None, window=None, sinks: int = 0, activation: str = "silu"):
+        self.norm_attention = RMSNorm(env, n)
+        self.attention = SelfAttention(env, n, heads, groups, head_dim, window, sinks)
+        self.norm_feed_forward = RMSNorm(env, n)
+        self.feed_forward = GatedFeedForward(env, n, n_hidden, activation)
+
+    def _feed_forward(self, x, attended, ctx):
+        y, total = self.norm_feed_forward.add(attended, x)
+        n = y.shape[-1]
+        return self.feed_forward.eval(y.reshape([y.shape[0] * y.shape[1], n]), ctx).reshape(y.shape) + total
+
+    def eval(self, x, ctx, length=None):
+        return self._feed_forward(x, self.attention.eval(self.norm_attention.eval(x, ctx), ctx, length), ctx)
+
+    def step(self, x: Array, cache: KeyValueCache, start: Array) -> Array:
+        ctx = EvalContext(False)
+        return self._feed_forward(x, self.attention.step(self.norm_attention.eval(x, ctx), cache, start), ctx)

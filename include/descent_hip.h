@@ -76,7 +76,18 @@ typedef enum dsc_kernel_kind {
     DSC_KERNEL_MATMUL = 3,           /* kernel.rs:386-557 + kernel_matmul.glsl */
     DSC_KERNEL_UNPAD = 4,            /* kernel.rs:645-710 */
     DSC_KERNEL_WINDOWS_TO_IMAGE = 5, /* kernel.rs:713-810 */
-    DSC_KERNEL_SCATTER_ADD = 6       /* kernel.rs:813-874 */
+    DSC_KERNEL_SCATTER_ADD = 6,      /* kernel.rs:813-874 */
+    /* Operators of sequence models (no counterpart in the reference, whose sequence model is the unrolled LSTM cell of
+       module.rs:281-363).  Operands and results are listed below at dsc_kernel_desc. */
+    DSC_KERNEL_RMS_NORM = 7,
+    DSC_KERNEL_RMS_NORM_GRAD = 8,
+    DSC_KERNEL_ROTARY = 9,
+    DSC_KERNEL_ATTENTION = 10,
+    DSC_KERNEL_ATTENTION_JOIN = 11,
+    DSC_KERNEL_ATTENTION_GRAD_QUERY = 12,
+    DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE = 13,
+    DSC_KERNEL_DUAL_MATMUL = 14,
+    DSC_KERNEL_GATED_GRAD = 15
 } dsc_kernel_kind;
 
 /* kernel.rs:8-35 `PerElementKernelOp` variants */
@@ -110,6 +121,10 @@ typedef enum dsc_compare_mode { DSC_CMP_EQ = 0, DSC_CMP_GT = 1 } dsc_compare_mod
 typedef enum dsc_reduce_op { DSC_REDUCE_MAX = 0, DSC_REDUCE_SUM = 1 } dsc_reduce_op;
 /* op.rs:76-80 */
 typedef enum dsc_matmul_output_mode { DSC_MATMUL_BATCHES = 0, DSC_MATMUL_ROWS = 1 } dsc_matmul_output_mode;
+/* operators: layout of a rotated pair, activation of a gated layer, what a dual product does with its two products */
+typedef enum dsc_rotary_layout { DSC_ROTARY_HALF = 0, DSC_ROTARY_INTERLEAVED = 1 } dsc_rotary_layout;
+typedef enum dsc_activation { DSC_ACT_SILU = 0, DSC_ACT_GELU = 1, DSC_ACT_RELU = 2, DSC_ACT_SIGMOID = 3 } dsc_activation;
+typedef enum dsc_dual_mode { DSC_DUAL_GATED = 0, DSC_DUAL_SUM = 1, DSC_DUAL_BOTH = 2 } dsc_dual_mode;
 
 typedef struct dsc_pe_op {
     int32_t kind;        /* dsc_pe_kind */
@@ -134,6 +149,33 @@ typedef struct dsc_pe_op {
  *   REDUCE/UNPAD/W2I  : [input, out]
  *   MATMUL            : [a, b, out]
  *   SCATTER_ADD       : [values, indices, accumulator(in/out)]
+ *   operators         : inputs[0..n_inputs), one buffer per entry of `outputs`, whose entries are indices into the
+ *                       operator's results in ascending order, the first result always among them
+ *
+ * Operators.  Views need no clamp; an operand marked (s) may have any non-negative strides with the elements of its
+ * last axis side by side (a DUAL_MATMUL operand: those of either axis), the others are dense.  Offsets are 64 bits wide.
+ * Sums, norms and softmax statistics are held in 32-bit floats; positions, starts and lengths are u32 words.
+ *   RMS_NORM       in  x [m,n] (s), weight [n], (residual [m,n] (s))            op_int {has residual}  op_float {epsilon}
+ *                  out 0: norm(sum) * weight [m,n]; 1: sum = x + residual [m,n]; 2: 1 / rms [m]
+ *   RMS_NORM_GRAD  in  sum [m,n] (s), 1 / rms [m], weight [n], d norm [m,n] (s), (d sum [m,n] (s))
+ *                  op_int {has d sum, partials p}      out 0: gradient of the sum [m,n]; 1: partial weight gradients [p,n]
+ *   ROTARY         in  x [batch,tokens,heads,dim] (s), frequencies [pairs], (positions [batch] or [batch,tokens])
+ *                  op_int {dsc_rotary_layout, inverse, rank of positions}  op_float {magnitude}     out 0: like x
+ *   ATTENTION      in  q [batch,tokens,heads,dim] (s), k, v [batch,keys,groups,dim] (s), (start [batch]), (length [batch])
+ *                  op_int {window or 0, sinks, 1: start given | 2: length given, splits}  op_float {scale}
+ *                  out 0: like q; 1: log of the softmax's denominator [batch,tokens,heads] (-inf where nothing is seen);
+ *                  with splits > 1 both have a leading axis of that extent and ATTENTION_JOIN makes them one
+ *   ATTENTION_JOIN in  the two of them     out 0: [batch,tokens,heads,dim]; 1: [batch,tokens,heads]
+ *   ATTENTION_GRAD_QUERY      in  q, k, v, out, d out (all s), log denominators, (start), (length); op_int, op_float as
+ *                  above without splits   out 0: dq; 1: sum over dim of out * d out [batch,tokens,heads]
+ *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (start), (length)   out 0: dk; 1: dv
+ *   DUAL_MATMUL    op_int {dsc_dual_mode, dsc_activation}
+ *                  GATED in a [m,k], b0, b1 [k,n] (s)        out 0: act(a b0) * (a b1) [m,n]; 1: a b0; 2: a b1
+ *                  SUM   in a0, a1 [m,k], b0, b1 [k,n] (s)   out 0: a0 b0 + a1 b1 [m,n]
+ *                  BOTH  in a [m,k], b0, b1 [k,n] (s)        out 0: a b0 [m,n]; 1: a b1
+ *                  A result that a non-finite operand element takes part in is NaN or infinite (which of the two may
+ *                  differ from what one chain of 32-bit multiply-adds gives); all other results are untouched by it.
+ *   GATED_GRAD     in  a b0, a b1, d out [m,n]               op_int {dsc_activation}       out 0: d (a b0); 1: d (a b1)
  */
 typedef struct dsc_kernel_desc {
     int32_t kind;            /* dsc_kernel_kind */
@@ -141,11 +183,11 @@ typedef struct dsc_kernel_desc {
     int32_t n_inputs;        /* number of input views below */
     const dsc_view* inputs;  /* PER_ELEMENT: per input; MATMUL: {a,b}; REDUCE/UNPAD/W2I: {input};
                                 SCATTER_ADD: {values, indices}; FILL: none */
-    /* PER_ELEMENT only */
+    /* PER_ELEMENT; operators use n_outputs and outputs */
     int32_t n_ops;
     const dsc_pe_op* ops;
     int32_t n_outputs;
-    const int32_t* outputs;  /* op index stored to each output (kernel.rs:199) */
+    const int32_t* outputs;  /* op index stored to each output (kernel.rs:199); operators: result index */
     int32_t n_builtin_views;
     const dsc_view* builtin_views;
     /* scalar attributes */
@@ -156,6 +198,8 @@ typedef struct dsc_kernel_desc {
     int32_t stride_w;        /* WINDOWS_TO_IMAGE (kernel.rs:716; tuple order is (w,h), kernel.rs:740) */
     int32_t stride_h;
     int32_t output_mode;     /* MATMUL: dsc_matmul_output_mode */
+    int32_t op_int[4];       /* operators: whole-number attributes, unused ones 0 */
+    uint32_t op_float[2];    /* operators: attributes as the bits of a float, unused ones 0 */
 } dsc_kernel_desc;
 
 /* ---------------------------------------------------------------- context */

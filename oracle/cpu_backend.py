@@ -14,6 +14,9 @@ import subprocess
 import numpy as np
 
 from descent_amd import _abi
+from descent_amd.operators import OperatorKernel
+
+from . import operators
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB_PATH = os.path.join(_HERE, "liboracle.so")
@@ -84,6 +87,11 @@ class CpuBackend:
 
     def launch(self, kernel, handles, rand_seed: int) -> None:
         self.launches.append(kernel.label_name())
+        if isinstance(kernel, OperatorKernel):
+            n = len(kernel.inputs)
+            for handle, value in zip(handles[n:], operators.evaluate(kernel, handles[:n])):
+                handle[:] = value.astype(np.float32).ravel()
+            return
         run_kernel(kernel, handles, rand_seed)
 
     def sync(self) -> None:

@@ -33,6 +33,15 @@ pub const DSC_KERNEL_MATMUL: i32 = 3;
 pub const DSC_KERNEL_UNPAD: i32 = 4;
 pub const DSC_KERNEL_WINDOWS_TO_IMAGE: i32 = 5;
 pub const DSC_KERNEL_SCATTER_ADD: i32 = 6;
+pub const DSC_KERNEL_RMS_NORM: i32 = 7;
+pub const DSC_KERNEL_RMS_NORM_GRAD: i32 = 8;
+pub const DSC_KERNEL_ROTARY: i32 = 9;
+pub const DSC_KERNEL_ATTENTION: i32 = 10;
+pub const DSC_KERNEL_ATTENTION_JOIN: i32 = 11;
+pub const DSC_KERNEL_ATTENTION_GRAD_QUERY: i32 = 12;
+pub const DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE: i32 = 13;
+pub const DSC_KERNEL_DUAL_MATMUL: i32 = 14;
+pub const DSC_KERNEL_GATED_GRAD: i32 = 15;
 
 // dsc_pe_kind
 pub const DSC_PE_LOAD: i32 = 0;
@@ -101,6 +110,8 @@ pub struct dsc_kernel_desc {
     pub stride_w: i32,
     pub stride_h: i32,
     pub output_mode: i32,
+    pub op_int: [i32; 4],
+    pub op_float: [u32; 2],
 }
 
 #[repr(C)]

@@ -145,6 +145,8 @@ impl MarshalledKernel {
             stride_w: 0,
             stride_h: 0,
             output_mode: 0,
+            op_int: [0; 4],
+            op_float: [0; 2],
         };
         let mut views = Vec::new();
         let mut ops = Vec::new();
