@@ -27,6 +27,7 @@ from .operators import (
     attention_ints,
     attention_splits,
     dual_matmul_shapes,
+    dual_matmul_splits,
     emit,
     norm_partials,
     norm_spec,
@@ -456,7 +457,7 @@ class Array:
         activation ("silu", "gelu", "relu" or "sigmoid") and the product of the two in one kernel."""
         w_gate, w_up = self._lift(w_gate), self._lift(w_up)
         dual_matmul_shapes(self.shape, w_gate.shape, w_up.shape, activation)
-        return emit([self, w_gate, w_up], OperatorSpec("DualMatMul", (DUAL_GATED, ACTIVATIONS.index(activation))), 1)[0]
+        return emit([self, w_gate, w_up], OperatorSpec("DualMatMul", (DUAL_GATED, ACTIVATIONS.index(activation), 1)), 1)[0]
 
 
 class DualArray:
@@ -768,11 +769,18 @@ class DualArray:
         wu, dwu = self._lift(w_up).into_inner()
         dual_matmul_shapes(x.shape, wg.shape, wu.shape, activation)
         act = ACTIVATIONS.index(activation)
-        h, gate, up = emit([x, wg, wu], OperatorSpec("DualMatMul", (DUAL_GATED, act)), 3)
+        h, gate, up = emit([x, wg, wu], OperatorSpec("DualMatMul", (DUAL_GATED, act, 1)), 3)
         h, dh = h.with_empty_grad()
         dgate, dup = emit([gate, up, dh], OperatorSpec("GatedGrad", (act,)), 2)
-        dx.accumulate(emit([dgate, dup, wg.transpose(), wu.transpose()], OperatorSpec("DualMatMul", (DUAL_SUM, 0)), 1)[0])
-        grad_gate, grad_up = emit([x.transpose(), dgate, dup], OperatorSpec("DualMatMul", (DUAL_BOTH, 0)), 2)
+        rows, width, hidden = x.shape[0], x.shape[1], wg.shape[1]
+
+        def product(operands, mode, m, n, k, count):
+            splits = dual_matmul_splits(m, n, k, mode)
+            results = emit(operands, OperatorSpec("DualMatMul", (mode, 0, splits)), count)
+            return [a if splits == 1 else a.reduce_sum(0, False) for a in results]
+
+        dx.accumulate(product([dgate, dup, wg.transpose(), wu.transpose()], DUAL_SUM, rows, width, hidden, 1)[0])
+        grad_gate, grad_up = product([x.transpose(), dgate, dup], DUAL_BOTH, width, hidden, rows, 2)
         dwg.accumulate(grad_gate)
         dwu.accumulate(grad_up)
         return DualArray(h, dh)

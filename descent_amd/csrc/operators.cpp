@@ -83,7 +83,8 @@ std::vector<dsc_shape> operator_results(const dsc_kernel_desc& d) {
     }
     case DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE: return {in[1].out_shape, in[2].out_shape};
     case DSC_KERNEL_DUAL_MATMUL: {
-        const dsc_shape out = shape_of({in[0].out_shape.dims[0], in[d.n_inputs - 1].out_shape.dims[1]});
+        const int64_t m = in[0].out_shape.dims[0], n = in[d.n_inputs - 1].out_shape.dims[1];
+        const dsc_shape out = d.op_int[2] > 1 ? shape_of({d.op_int[2], m, n}) : shape_of({m, n});
         if (d.op_int[0] == DSC_DUAL_GATED) return {out, out, out};
         if (d.op_int[0] == DSC_DUAL_SUM) return {out};
         return {out, out};
@@ -189,6 +190,7 @@ string validate_operator(const dsc_kernel_desc& d) {
     }
     case DSC_KERNEL_DUAL_MATMUL: {
         if (op[0] < 0 || op[0] > 2 || op[1] < 0 || op[1] > 3) return name + "unknown mode or activation";
+        if (op[2] < 1 || op[2] > 64 || (op[0] == DSC_DUAL_GATED && op[2] != 1)) return name + "between 1 and 64 splits, one for a gated product";
         const bool sum = op[0] == DSC_DUAL_SUM;
         if (d.n_inputs != (sum ? 4 : 3)) return name + "wrong number of operands";
         for (int i = 0; i < d.n_inputs; ++i)
@@ -460,7 +462,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     const int mode = d.op_int[0];
     const bool sum = mode == DSC_DUAL_SUM, paired = !sum;
     const int b = sum ? 2 : 1;
-    const int64_t m = d.shape.dims[0], n = d.shape.dims[1], k = d.inputs[0].out_shape.dims[1];
+    const int64_t m = d.inputs[0].out_shape.dims[0], n = d.inputs[b].out_shape.dims[1], k = d.inputs[0].out_shape.dims[1];
     const int a_of[2] = {0, sum ? 1 : 0}, b_of[2] = {b, b + 1};
     const char* names[4] = {"DM_A0", "DM_A1", "DM_B0", "DM_B1"};
     bool a_kc = true, b_kc = true, a_vec = true, b_vec = true, b_rows = true;
@@ -482,7 +484,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     def.set("DM_K", k);
     const string size = "_m" + to_string((long long)m) + "_n" + to_string((long long)n) + "_k" + to_string((long long)k);
     g->algo_flops = 4.0 * (double)m * (double)n * (double)k;
-    g->algo_bytes = 4.0 * ((double)m * (double)k * (sum ? 2 : 1) + 2.0 * (double)k * (double)n + (double)m * (double)n * d.n_outputs);
+    g->algo_bytes = 4.0 * ((double)m * (double)k * (sum ? 2 : 1) + 2.0 * (double)k * (double)n + (double)m * (double)n * d.n_outputs * d.op_int[2]);
     const std::vector<string> operands = {input_arg(fk, 0), input_arg(fk, sum ? 1 : 0), input_arg(fk, b), input_arg(fk, b + 1)};
     std::vector<string> args = operands;
     for (int i = 0; i < 3; ++i) args.push_back(result_arg(fk, i));
@@ -495,35 +497,37 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
         g->note = "columns x32, k in 128 slices";
         return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_few" + size, "gated_few_rows", args, up(n, 32), 1024, 1, g);
     }
-    // tile: the largest that still gives every CU a workgroup
+    // Tile.  A CU's step of 16 k costs 2.4 us with 256x256 (8 waves of 128x64), 0.73 with 128x128 (8 waves of 32x64; with 4
+    // waves of 64x64 0.83) and, alone on its CU, 0.55 with 64x64: the largest tile that leaves no CU without one, and
+    // the smallest where even that many do not fill the CUs (1001 x 1366 columns x 512 k of both products: 32 us with
+    // 128x128, 37 with 64x64; 1001 x 500, k 2 x 1366, not split: 113 and 98).
     struct Tile {
-        int bm, bn, wm, wn;
+        int bm, bn, wm, wn, ahead;
     };
-    const Tile tiles[] = {{128, 128, 2, 2}, {64, 128, 2, 2}, {64, 64, 2, 1}};
-    Tile t = tiles[2];
-    if (m <= 32) t = {32, 128, 1, 2};
-    else
-        for (const Tile& c : tiles)
-            if (up(m, c.bm) * up(n, paired ? c.bn / 2 : c.bn) >= 256) {
-                t = c;
-                break;
-            }
+    const int64_t splits = d.op_int[2];
+    auto count = [&](int bm, int bn) { return up(m, bm) * up(n, paired ? bn / 2 : bn) * splits; };
+    Tile t = {128, 128, 4, 2, 2};
+    if (m <= 32) t = {32, 128, 1, 2, 4};
+    else if (count(256, 256) >= 256) t = {256, 256, 2, 4, 2};
+    else if (count(64, 64) <= 256) t = {64, 64, 2, 1, 4};
     const int64_t tiles_m = up(m, t.bm), tiles_n = up(n, paired ? t.bn / 2 : t.bn);
-    if (tiles_m * tiles_n >= (int64_t(1) << 30)) return "kernel too large: more than 2^30 tiles";
+    if (tiles_m * tiles_n * splits >= (int64_t(1) << 30)) return "kernel too large: more than 2^30 tiles";
     def.set("DM_BM", t.bm);
     def.set("DM_BN", t.bn);
     def.set("DM_WM", t.wm);
     def.set("DM_WN", t.wn);
+    def.set("DM_AHEAD", t.ahead);
+    def.set("DM_SPLITS", splits);
     def.set("DM_A_KC", a_kc ? 1 : 0);
     def.set("DM_B_KC", b_kc ? 1 : 0);
-    def.set("DM_A_VEC", a_vec ? 1 : 0);
-    def.set("DM_B_VEC", b_vec ? 1 : 0);
+    def.set("DM_A_VEC", a_vec && k % 4 == 0 ? 1 : 0);  // (quads that are moved back to end with k keep their alignment)
+    def.set("DM_B_VEC", b_vec && k % 4 == 0 ? 1 : 0);
     def.set("DM_TILES_M", tiles_m);
     def.set("DM_TILES_N", tiles_n);
     def.set("DM_GROUP", 8);
-    g->note = "bf16x6 32x32x16 tile " + to_string(t.bm) + "x" + to_string(t.bn) + "x32 waves " + to_string(t.wm) + "x" + to_string(t.wn) + " A" +
+    g->note = "bf16x6 32x32x16 tile " + to_string(t.bm) + "x" + to_string(t.bn) + "x16 waves " + to_string(t.wm) + "x" + to_string(t.wn) + " A" +
               (a_kc ? a_vec ? "k4" : "k1" : "r") + " B" + (b_kc ? b_vec ? "k4" : "k1" : "r");
-    return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_" + what + size, "dual_matmul", args, up(tiles_m * tiles_n, 8) * 8, 64 * t.wm * t.wn, 2, g);
+    return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_" + what + size, "dual_matmul", args, up(tiles_m * tiles_n * splits, 8) * 8, 64 * t.wm * t.wn, 2, g);
 }
 
 }  // namespace

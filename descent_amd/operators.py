@@ -36,7 +36,7 @@ class OperatorSpec:
     Attention              ints (window, sinks, 1 start | 2 length, splits)   floats (scale,)
     AttentionJoin          -
     AttentionGrad*         ints (window, sinks, 1 start | 2 length)      floats (scale,)
-    DualMatMul             ints (mode, activation)
+    DualMatMul             ints (mode, activation, splits)
     GatedGrad              ints (activation,)
     """
 
@@ -71,8 +71,8 @@ class OperatorSpec:
         if name == "AttentionGradKeyValue":
             return [shapes[1], shapes[2]]
         if name == "DualMatMul":
-            mode = self.ints[0]
-            out = Shape((shapes[0][0], shapes[-1][1]))
+            mode, _, splits = self.ints
+            out = Shape(((splits,) if splits > 1 else ()) + (shapes[0][0], shapes[-1][1]))
             return {DUAL_GATED: [out] * 3, DUAL_SUM: [out], DUAL_BOTH: [out] * 2}[mode]
         assert name == "GatedGrad"
         return [shapes[0], shapes[0]]
@@ -248,3 +248,13 @@ def dual_matmul_shapes(x: Shape, w_gate: Shape, w_up: Shape, activation: str) ->
     _need(len(w_gate) == 2 and tuple(w_gate) == tuple(w_up) and w_gate[0] == x[1],
           f"gated_dense: weights {w_gate!r} and {w_up!r} must both be [{x[1]}, hidden]")
     _need(activation in ACTIVATIONS, f"gated_dense: activation must be one of {ACTIVATIONS}, got {activation!r}")
+
+
+def dual_matmul_splits(rows: int, columns: int, k: int, mode: int) -> int:
+    """Pieces of the k range of a gradient's product.  Where the result is small its tiles (128 rows by 128 columns, or 64
+    of each of two products) are too few for 256 CUs: k is then cut into up to 8 pieces of 12 steps of 16 or more, until
+    there are 384 workgroups, and a Reduce sums the pieces.  Measured: 1001 x 500 over k 2 x 1366 113 us whole, 27 in 8
+    pieces; 500 x 1366 (two results) over k 1001 52 us whole, 31 in 4."""
+    tiles = (rows + 127) // 128 * ((columns + 127) // 128 if mode == DUAL_SUM else (columns + 63) // 64)
+    steps = (k + 15) // 16 * (2 if mode == DUAL_SUM else 1)
+    return max(1, min(384 // tiles, steps // 12, 8))

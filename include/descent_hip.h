@@ -169,7 +169,8 @@ typedef struct dsc_pe_op {
  *   ATTENTION_GRAD_QUERY      in  q, k, v, out, d out (all s), log denominators, (start), (length); op_int, op_float as
  *                  above without splits   out 0: dq; 1: sum over dim of out * d out [batch,tokens,heads]
  *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (start), (length)   out 0: dk; 1: dv
- *   DUAL_MATMUL    op_int {dsc_dual_mode, dsc_activation}
+ *   DUAL_MATMUL    op_int {dsc_dual_mode, dsc_activation, splits}; with splits > 1 (SUM and BOTH) the k range is cut into
+ *                  that many pieces and the results have a leading axis of that extent, to be summed over
  *                  GATED in a [m,k], b0, b1 [k,n] (s)        out 0: act(a b0) * (a b1) [m,n]; 1: a b0; 2: a b1
  *                  SUM   in a0, a1 [m,k], b0, b1 [k,n] (s)   out 0: a0 b0 + a1 b1 [m,n]
  *                  BOTH  in a [m,k], b0, b1 [k,n] (s)        out 0: a b0 [m,n]; 1: a b1

@@ -173,6 +173,8 @@ def evaluate(kernel, arrays):
             got = x[0] @ x[1], x[0] @ x[2]
         else:
             got = (x[0] @ x[2] + x[1] @ x[3],)
+        if ints[2] > 1:  # the whole sum as the first piece: what is made of the pieces is their sum
+            got = [np.concatenate([a[None], np.zeros((ints[2] - 1,) + a.shape)]) for a in got]
     else:
         assert name == "GatedGrad"
         a, slope = activation(ACTIVATIONS[ints[0]], x[0])

@@ -237,7 +237,7 @@ DUALS = [(DUAL_GATED, 1, 1, 1, 0), (DUAL_GATED, 1, 4096, 200, 0), (DUAL_GATED, 3
          (DUAL_BOTH, 1, 1, 1, 0), (DUAL_BOTH, 70, 129, 35, 0), (DUAL_BOTH, 33, 64, 200, 0), (DUAL_BOTH, 1030, 1100, 36, 0), (DUAL_BOTH, 400, 300, 70, 0)]
 
 
-def dual_case(mode, rows, columns, k, act, rng, transposed=()):
+def dual_case(mode, rows, columns, k, act, rng, transposed=(), splits=1):
     """`transposed`: operands that are read through a transposing view."""
     left = 2 if mode == DUAL_SUM else 1
     shapes = [(rows, k)] * left + [(k, columns)] * 2
@@ -249,14 +249,14 @@ def dual_case(mode, rows, columns, k, act, rng, transposed=()):
         else:
             arrays.append(normal(rng, *s))
             views.append(Shape(s).identity_view())
-    return kernel(OperatorSpec("DualMatMul", (mode, act)), arrays, views), arrays
+    return kernel(OperatorSpec("DualMatMul", (mode, act, splits)), arrays, views), arrays
 
 
 def dual_bounds(k, arrays, want):
     """Each of the six products of parts is added with one rounding: 6 k of them, each at most U times the sum of the
     products' magnitudes, and the products left out are below 4 U of them together."""
     x = [np.abs(ref.through(v, a).astype(np.float64)) for v, a in zip(k.inputs, flat(arrays))]
-    mode, act = k.spec.ints
+    mode, act, _ = k.spec.ints
     n = x[0].shape[1]
     step = (6 * n + 4) * U
     if mode == DUAL_BOTH:

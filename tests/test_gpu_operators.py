@@ -105,6 +105,18 @@ def test_dual_product(hip_backend_session, case):
     check(hip_backend_session, *cases.dual_case(*case, rng, transposed=(left,)), cases.dual_bounds)
 
 
+@pytest.mark.parametrize("splits", [2, 7, 64])
+@pytest.mark.parametrize("case", [c for c in cases.DUALS if c[0] != DUAL_GATED and c[1] < 2000], ids=str)
+def test_dual_product_in_pieces(hip_backend_session, case, splits):
+    """More pieces than steps leave some empty; the sum over the pieces is the product."""
+    kernel, arrays = cases.dual_case(*case, np.random.default_rng(17), splits=splits)
+    whole = cases.kernel(OperatorSpec("DualMatMul", kernel.spec.ints[:2] + (1,)), arrays)
+    want = ref.evaluate(whole, cases.flat(arrays))
+    for g, w, b in zip(launch(hip_backend_session, kernel, arrays), want, cases.dual_bounds(whole, arrays, want)):
+        assert g.shape[0] == splits
+        assert (np.abs(g.astype(np.float64).sum(0) - w) <= b + cases.U * np.abs(w)).all()
+
+
 @pytest.mark.parametrize("rows", [4, 40, 300])
 @pytest.mark.parametrize("mode", [DUAL_GATED, DUAL_SUM, DUAL_BOTH])
 def test_dual_product_keeps_all_bits(hip_backend_session, mode, rows):

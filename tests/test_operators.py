@@ -327,10 +327,10 @@ def test_malformed_operator_descriptors_are_rejected_with_a_message():
         OperatorKernel(OperatorSpec("AttentionGradQuery", (0, 0, 0), (1.0,)), (q, k, k, q, q, ident(2, 5, 3)), (0,)),
         OperatorKernel(OperatorSpec("AttentionGradKeyValue", (0, 0, 0), (1.0,)), (q, k, k, k, ident(2, 5, 4), ident(2, 5, 4)), (0,)),
         OperatorKernel(OperatorSpec("AttentionJoin"), (ident(3, 2, 5, 4, 8), ident(2, 2, 5, 4)), (0,)),
-        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_GATED, 4)), (ident(3, 4), ident(4, 5), ident(4, 5)), (0,)),
-        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0)), (ident(3, 4), ident(5, 5), ident(5, 5)), (0,)),
-        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_SUM, 0)), (ident(3, 4), ident(2, 4), ident(4, 5), ident(4, 5)), (0,)),
-        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0)), (_view((6, 8), mapping=((0, 2), (1, 2)), out=(3, 4)), ident(4, 5), ident(4, 5)), (0,)),
+        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_GATED, 4, 1)), (ident(3, 4), ident(4, 5), ident(4, 5)), (0,)),
+        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0, 1)), (ident(3, 4), ident(5, 5), ident(5, 5)), (0,)),
+        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_SUM, 0, 1)), (ident(3, 4), ident(2, 4), ident(4, 5), ident(4, 5)), (0,)),
+        OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0, 1)), (_view((6, 8), mapping=((0, 2), (1, 2)), out=(3, 4)), ident(4, 5), ident(4, 5)), (0,)),
         OperatorKernel(OperatorSpec("GatedGrad", (4,)), (ident(3, 4),) * 3, (0,)),
         OperatorKernel(OperatorSpec("GatedGrad", (0,)), (ident(3, 4), ident(3, 4), ident(4, 3)), (0,)),
     ]
@@ -339,7 +339,7 @@ def test_malformed_operator_descriptors_are_rejected_with_a_message():
             hip_backend.codegen_source(kernel)
         assert e.value.status == _abi.ERR_INVALID and len(str(e.value)) > 20, (i, str(e.value))
     # attributes that the Python classes cannot hold
-    good = [(att((0, 0, 0, 1), (q, k, k)), 3, 0), (OperatorKernel(OperatorSpec("DualMatMul", (0, 0)), (ident(3, 4), ident(4, 5), ident(4, 5)), (0,)), 0, 3),
+    good = [(att((0, 0, 0, 1), (q, k, k)), 3, 0), (OperatorKernel(OperatorSpec("DualMatMul", (0, 0, 1)), (ident(3, 4), ident(4, 5), ident(4, 5)), (0,)), 0, 3),
             (OperatorKernel(OperatorSpec("RmsNormGrad", (0, 1)), (ident(4, 6), ident(4), ident(6), ident(4, 6)), (0,)), 1, 0)]
     for kernel, at, value in good:
         mk = _abi.MarshalledKernel(kernel)
