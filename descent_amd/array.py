@@ -32,6 +32,7 @@ from .operators import (
     norm_partials,
     norm_spec,
     rotary_spec,
+    sink_pieces,
 )
 from .shape import BATCHES, ROWS, Shape, View
 
@@ -757,7 +758,10 @@ class DualArray:
         out, dout = out.with_empty_grad()
         places = [a for a in (start, length) if a is not None]
         grad_q, delta = emit([q, k, v, out, dout, lse] + places, OperatorSpec("AttentionGradQuery", ints, (scale,)), 2)
-        grad_k, grad_v = emit([q, k, v, dout, lse, delta] + places, OperatorSpec("AttentionGradKeyValue", ints, (scale,)), 2)
+        pieces = sink_pieces(q.shape, k.shape, window, ints[1])
+        rows = [q, k, v, dout, lse, delta]
+        far = emit(rows + places, OperatorSpec("AttentionGradSinks", ints + (pieces,), (scale,)), 2) if pieces else []
+        grad_k, grad_v = emit(rows + far + places, OperatorSpec("AttentionGradKeyValue", ints + (pieces,), (scale,)), 2)
         dq.accumulate(grad_q)
         dk.accumulate(grad_k)
         dv.accumulate(grad_v)

@@ -13,7 +13,7 @@ using std::string;
 using std::to_string;
 
 const char* const kNames[] = {"RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionJoin", "AttentionGradQuery", "AttentionGradKeyValue",
-                              "DualMatMul", "GatedGrad"};
+                              "DualMatMul", "GatedGrad", "AttentionGradSinks"};
 
 float as_float(uint32_t bits) {
     float f;
@@ -82,6 +82,11 @@ std::vector<dsc_shape> operator_results(const dsc_kernel_desc& d) {
         return {in[0].out_shape, shape_of({q[0], q[1], q[2]})};
     }
     case DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE: return {in[1].out_shape, in[2].out_shape};
+    case DSC_KERNEL_ATTENTION_GRAD_SINKS: {
+        const int64_t* k = in[1].out_shape.dims;
+        const dsc_shape far = shape_of({d.op_int[3], k[0], std::min<int64_t>(d.op_int[1], k[1]), k[2], k[3]});
+        return {far, far};
+    }
     case DSC_KERNEL_DUAL_MATMUL: {
         const int64_t m = in[0].out_shape.dims[0], n = in[d.n_inputs - 1].out_shape.dims[1];
         const dsc_shape out = d.op_int[2] > 1 ? shape_of({d.op_int[2], m, n}) : shape_of({m, n});
@@ -154,8 +159,10 @@ string validate_operator(const dsc_kernel_desc& d) {
     }
     case DSC_KERNEL_ATTENTION:
     case DSC_KERNEL_ATTENTION_GRAD_QUERY:
+    case DSC_KERNEL_ATTENTION_GRAD_SINKS:
     case DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE: {
-        const int arrays = d.kind == DSC_KERNEL_ATTENTION ? 3 : 6;
+        const bool joins = d.kind == DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE && op[3] != 0;
+        const int arrays = d.kind == DSC_KERNEL_ATTENTION ? 3 : joins ? 8 : 6;
         if (op[2] < 0 || op[2] > 3 || d.n_inputs != arrays + (op[2] & 1) + (op[2] >> 1)) return name + "wrong number of operands";
         if (!ranks({4, 4, 4})) return name + "queries, keys and values have four axes";
         const int64_t *q = dims(0), *k = dims(1);
@@ -177,6 +184,10 @@ string validate_operator(const dsc_kernel_desc& d) {
         } else {
             if (!same_shape(in[3].out_shape, in[0].out_shape) || !is_shape(in[4].out_shape, {q[0], q[1], q[2]}) || !is_shape(in[5].out_shape, {q[0], q[1], q[2]}))
                 return name + "the output's gradient or the rows' sums do not fit";
+            if (op[3] < 0 || op[3] > 64 || (d.kind == DSC_KERNEL_ATTENTION_GRAD_SINKS && op[3] == 0)) return name + "between 1 and 64 pieces";
+            if (op[3] && (op[0] == 0 || op[1] == 0)) return name + "pieces without a window and sinks";
+            for (int i = 6; joins && i < 8; ++i)
+                if (!is_shape(in[i].out_shape, {op[3], k[0], std::min<int64_t>(op[1], k[1]), k[2], k[3]})) return name + "the sinks' pieces do not fit";
             e = views({0, 1, 2, 3}, false);
         }
         break;
@@ -411,7 +422,9 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
         def.set64(string(s.first) + "_H", o.stride[2]);
     }
     def.set("AT_VEC", quads ? 1 : 0);
-    const int arrays = forward ? 3 : 6;
+    const bool sinks = d.kind == DSC_KERNEL_ATTENTION_GRAD_SINKS, joins = !forward && !grad_q && !sinks && op[3];
+    def.set("AT_PIECES", forward || grad_q ? 0 : op[3]);
+    const int arrays = forward ? 3 : joins ? 8 : 6;
     const string start = op[2] & 1 ? input_arg(fk, arrays, true) : "(const uint*)nullptr";
     const string length = op[2] & 2 ? input_arg(fk, arrays + (op[2] & 1), true) : "(const uint*)nullptr";
     const string size = "_b" + to_string((long long)q[0]) + "_t" + to_string((long long)q[1]) + "_s" + to_string((long long)k[1]) + "_h" +
@@ -437,11 +450,20 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
                          result_arg(fk, 0), result_arg(fk, 1)},
                         q[0] * k[2] * up(rows, 64), 256, waves, g);
     }
+    if (sinks) {
+        def.set("AT_GRAD_SINKS", 1);
+        return assemble(fk, def, kAttentionSource, "dsc_attention_grad_sinks" + size, "attention_grad_sinks",
+                        {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), input_arg(fk, 3), input_arg(fk, 4), input_arg(fk, 5), start, length,
+                         result_arg(fk, 0), result_arg(fk, 1)},
+                        q[0] * k[2] * up(std::min<int64_t>(op[1], k[1]), 16) * op[3], 256, waves, g);
+    }
     def.set("AT_GRAD_KEY_VALUE", 1);
+    def.set("AT_HALVES", waves);
     return assemble(fk, def, kAttentionSource, "dsc_attention_grad_key_value" + size, "attention_grad_key_value",
-                    {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), input_arg(fk, 3), input_arg(fk, 4), input_arg(fk, 5), start, length,
+                    {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), input_arg(fk, 3), input_arg(fk, 4), input_arg(fk, 5),
+                     joins ? input_arg(fk, 6) : "(const float*)nullptr", joins ? input_arg(fk, 7) : "(const float*)nullptr", start, length,
                      result_arg(fk, 0), result_arg(fk, 1)},
-                    q[0] * k[2] * up(k[1], 64), 256, waves, g);
+                    q[0] * k[2] * up(k[1], 64), 256 * waves, waves, g);
 }
 
 string gen_dual_matmul(const FusedKernel& fk, Generated* g) {

@@ -18,7 +18,7 @@ from .shape import Shape, View
 # kinds, in the order of dsc_kernel_kind from DSC_KERNEL_RMS_NORM on
 OPERATORS = (
     "RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionJoin", "AttentionGradQuery", "AttentionGradKeyValue",
-    "DualMatMul", "GatedGrad",
+    "DualMatMul", "GatedGrad", "AttentionGradSinks",
 )
 ACTIVATIONS = ("silu", "gelu", "relu", "sigmoid")
 LAYOUTS = ("half", "interleaved")
@@ -35,7 +35,8 @@ class OperatorSpec:
     Rotary                 ints (layout, inverse, positions rank)        floats (magnitude,)
     Attention              ints (window, sinks, 1 start | 2 length, splits)   floats (scale,)
     AttentionJoin          -
-    AttentionGrad*         ints (window, sinks, 1 start | 2 length)      floats (scale,)
+    AttentionGradQuery     ints (window, sinks, 1 start | 2 length)      floats (scale,)
+    AttentionGradSinks, AttentionGradKeyValue   the same and pieces
     DualMatMul             ints (mode, activation, splits)
     GatedGrad              ints (activation,)
     """
@@ -68,6 +69,9 @@ class OperatorSpec:
             return [Shape(shapes[0][1:]), Shape(shapes[1][1:])]
         if name == "AttentionGradQuery":
             return [shapes[0], Shape(shapes[0][:3])]
+        if name == "AttentionGradSinks":
+            b, keys, groups, dim = shapes[1]
+            return [Shape((self.ints[3], b, min(self.ints[1], keys), groups, dim))] * 2
         if name == "AttentionGradKeyValue":
             return [shapes[1], shapes[2]]
         if name == "DualMatMul":
@@ -89,7 +93,7 @@ class OperatorSpec:
             return "rows" if arg < 3 else "dense"
         if name == "AttentionGradQuery":
             return "rows" if arg < 5 else "dense"
-        if name == "AttentionGradKeyValue":
+        if name in ("AttentionGradSinks", "AttentionGradKeyValue"):
             return "rows" if arg < 4 else "dense"
         if name in ("RmsNorm", "RmsNormGrad"):
             wide = {"RmsNorm": (0, 2), "RmsNormGrad": (0, 3, 4)}[name]
@@ -241,6 +245,15 @@ def attention_splits(q: Shape, k: Shape, window, sinks: int) -> int:
         return 1
     reach = k[1] if window is None else min(k[1], window + sinks + tokens)
     return max(1, min(512 // workgroups, reach // 256, 64))
+
+
+def sink_pieces(q: Shape, k: Shape, window, sinks: int) -> int:
+    """Pieces of 256 rows that the rows beyond a window's length are cut into for the sinks' gradients (0: no kernel of
+    their own, fewer than two pieces)."""
+    if not window or not sinks:
+        return 0
+    rows = max(0, q[1] - window) * (q[2] // k[2])
+    return 0 if rows <= 256 else min((rows + 255) // 256, 64)
 
 
 def dual_matmul_shapes(x: Shape, w_gate: Shape, w_up: Shape, activation: str) -> None:

@@ -87,7 +87,8 @@ typedef enum dsc_kernel_kind {
     DSC_KERNEL_ATTENTION_GRAD_QUERY = 12,
     DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE = 13,
     DSC_KERNEL_DUAL_MATMUL = 14,
-    DSC_KERNEL_GATED_GRAD = 15
+    DSC_KERNEL_GATED_GRAD = 15,
+    DSC_KERNEL_ATTENTION_GRAD_SINKS = 16
 } dsc_kernel_kind;
 
 /* kernel.rs:8-35 `PerElementKernelOp` variants */
@@ -168,7 +169,12 @@ typedef struct dsc_pe_op {
  *   ATTENTION_JOIN in  the two of them     out 0: [batch,tokens,heads,dim]; 1: [batch,tokens,heads]
  *   ATTENTION_GRAD_QUERY      in  q, k, v, out, d out (all s), log denominators, (start), (length); op_int, op_float as
  *                  above without splits   out 0: dq; 1: sum over dim of out * d out [batch,tokens,heads]
- *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (start), (length)   out 0: dk; 1: dv
+ *   ATTENTION_GRAD_SINKS      in  q, k, v, d out (all s), log denominators, that sum, (start), (length)
+ *                  op_int {window, sinks, as above, pieces}   out 0, 1: [pieces,batch,sinks,groups,dim], what the rows past
+ *                  the window of a tile of 64 keys add to its sinks' dk (not yet scaled) and dv
+ *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (those two), (start), (length)
+ *                  op_int {window, sinks, as above, pieces or 0: the two are not given and nothing is left out}
+ *                  out 0: dk; 1: dv
  *   DUAL_MATMUL    op_int {dsc_dual_mode, dsc_activation, splits}; with splits > 1 (SUM and BOTH) the k range is cut into
  *                  that many pieces and the results have a leading axis of that extent, to be summed over
  *                  GATED in a [m,k], b0, b1 [k,n] (s)        out 0: act(a b0) * (a b1) [m,n]; 1: a b0; 2: a b1

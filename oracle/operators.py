@@ -87,12 +87,14 @@ def attention(q, k, v, window, sinks, scale, start=None, length=None):
     return out, lse
 
 
-def attention_grad(q, k, v, out, dout, lse, window, sinks, scale, start=None, length=None):
-    """dq, dk, dv and delta = sum(out * dout)."""
+def attention_grad(q, k, v, out, dout, lse, window, sinks, scale, start=None, length=None, pick=None):
+    """dq, dk, dv and delta = sum(out * dout).  `pick(sequence, tokens)` limits the pairs that count."""
     b, t, h, d = q.shape
     dq, dk, dv, delta = np.zeros_like(q), np.zeros_like(k), np.zeros_like(v), np.zeros((b, t, h))
     for i, j, g, first, count in _each_head(q, k, start, length):
         sees = visible(t, k.shape[1], window, sinks, first, count)
+        if pick is not None:
+            sees = sees & pick(i, t)
         for r in np.nonzero(sees.any(1))[0]:
             at = np.nonzero(sees[r])[0]
             with np.errstate(invalid="ignore"):
@@ -135,8 +137,9 @@ def evaluate(kernel, arrays):
         got = ds, np.stack([share[p :: ints[1]].sum(0) for p in range(ints[1])])
     elif name == "Rotary":
         got = (rotary(x[0], raw[1], whole[2] if ints[2] else None, ints[0], float(np.float32(floats[0])), ints[1]),)
-    elif name in ("Attention", "AttentionGradQuery", "AttentionGradKeyValue"):
-        places = whole[3 if name == "Attention" else 6 :]
+    elif name in ("Attention", "AttentionGradQuery", "AttentionGradKeyValue", "AttentionGradSinks"):
+        joins = name == "AttentionGradKeyValue" and ints[3] > 0
+        places = whole[3 if name == "Attention" else 8 if joins else 6 :]
         start = places[0] if ints[2] & 1 else None
         length = places[-1] if ints[2] & 2 else None
         scale = float(np.float32(floats[0]))
@@ -154,8 +157,26 @@ def evaluate(kernel, arrays):
             q, k, v, dout, lse, delta = x[:6]
             square = (dout * dout).sum(-1, keepdims=True)
             out = np.where(square > 0, dout * delta[..., None] / np.where(square > 0, square, 1.0), 0.0)
-            _, dk, dv, _ = attention_grad(q, k, v, out, dout, lse, ints[0], ints[1], scale, start, length)
-            got = dk, dv
+            if joins or name == "AttentionGradSinks":  # rows at this place or past it belong to the sinks' kernel
+                def far(i, t):
+                    place = (int(start[i]) if start is not None else k.shape[1] - t) + np.arange(t)
+                    return place[:, None] >= np.minimum(np.arange(k.shape[1]) // 64 * 64 + 63, k.shape[1] - 1) + ints[0]
+
+                pick = far if name == "AttentionGradSinks" else lambda i, t: ~far(i, t)
+            else:
+                pick = None
+            _, dk, dv, _ = attention_grad(q, k, v, out, dout, lse, ints[0], ints[1], scale, start, length, pick)
+            if name == "AttentionGradSinks":
+                sinks = min(ints[1], k.shape[1])
+                got = [np.concatenate([a[None, :, :sinks], np.zeros((ints[3] - 1,) + a[:, :sinks].shape)]) for a in (dk / scale, dv)]
+            else:
+                if joins:
+                    sinks = x[6].shape[2]
+                    dk[:, :sinks] += x[6].sum(0) * scale
+                    dv[:, :sinks] += x[7].sum(0)
+                    for i in range(k.shape[0] if length is not None else 0):  # keys past the length get no gradient
+                        dk[i, int(length[i]) :] = dv[i, int(length[i]) :] = 0.0
+                got = dk, dv
     elif name == "AttentionJoin":
         part, lse = x
         top = lse.max(0)

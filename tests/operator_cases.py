@@ -165,8 +165,8 @@ def attention_bounds(k, arrays, want):
     return [out, lse]
 
 
-def attention_grad_cases(batch, tokens, keys, heads, groups, dim, window, sinks, places, rng):
-    """Both gradient kernels, on the 64-bit forward results rounded to 32."""
+def attention_grad_cases(batch, tokens, keys, heads, groups, dim, window, sinks, places, rng, pieces=0):
+    """The gradient kernels (with `pieces` those that share the sinks' rows, too), on the 64-bit forward results rounded to 32."""
     k, arrays = attention_case(batch, tokens, keys, heads, groups, dim, window, sinks, places, rng)
     out, lse = (a.astype(np.float32) for a in ref.evaluate(k, flat(arrays)))
     dout = normal(rng, *out.shape, scale=0.5)
@@ -174,8 +174,14 @@ def attention_grad_cases(batch, tokens, keys, heads, groups, dim, window, sinks,
     delta = (out.astype(np.float64) * dout).sum(-1).astype(np.float32)
     by_query = arrays[:3] + [out, dout, lse] + tail
     by_key = arrays[:3] + [dout, lse, delta] + tail
-    return [(kernel(OperatorSpec("AttentionGradQuery", ints, floats), by_query), by_query),
-            (kernel(OperatorSpec("AttentionGradKeyValue", ints, floats), by_key), by_key)]
+    cases = [(kernel(OperatorSpec("AttentionGradQuery", ints, floats), by_query), by_query),
+             (kernel(OperatorSpec("AttentionGradKeyValue", ints + (0,), floats), by_key), by_key)]
+    if pieces:
+        far = kernel(OperatorSpec("AttentionGradSinks", ints + (pieces,), floats), by_key)
+        some = [normal(rng, *s) for s in far.result_shapes()]
+        joined = by_key[:6] + some + tail
+        cases += [(far, by_key), (kernel(OperatorSpec("AttentionGradKeyValue", ints + (pieces,), floats), joined), joined)]
+    return cases
 
 
 def attention_grad_bounds(k, arrays, want):
@@ -188,7 +194,8 @@ def attention_grad_bounds(k, arrays, want):
     out = arrays[3].astype(np.float64) if by_query else None
     heads, groups, dim = q.shape[2], key.shape[2], q.shape[3]
     dq, delta, dk, dv = np.zeros(q.shape), np.zeros(lse.shape), np.zeros(key.shape), np.zeros(key.shape)
-    for i, j, g, sees in _pairs(k, arrays, 6):
+    joins = not by_query and k.spec.name == "AttentionGradKeyValue" and k.spec.ints[3]
+    for i, j, g, sees in _pairs(k, arrays, 8 if joins else 6):
         real = scale * q[i, :, j] @ key[i, :, g].T
         size = scale * np.abs(q[i, :, j]) @ np.abs(key[i, :, g]).T
         row = np.where(np.isfinite(lse[i, :, j]), lse[i, :, j], 0.0)
@@ -208,6 +215,13 @@ def attention_grad_bounds(k, arrays, want):
         rows = heads // groups * sees.sum(0)[:, None] + 4
         dk[i, :, g] += scale * (ds_off.T @ np.abs(q[i, :, j]) + rows * U * (ds.T @ np.abs(q[i, :, j])))
         dv[i, :, g] += (p * off).T @ np.abs(dout[i, :, j]) + rows * U * (p.T @ np.abs(dout[i, :, j]))
+    if k.spec.name == "AttentionGradSinks":  # any piece may hold any of the rows
+        sinks = want[0].shape[2]
+        return [np.broadcast_to(a[None, :, :sinks], want[0].shape) for a in (dk / scale, dv)]
+    if joins:
+        sinks, n = arrays[6].shape[2], arrays[6].shape[0] + 2
+        dk[:, :sinks] += scale * n * U * np.abs(arrays[6].astype(np.float64)).sum(0)
+        dv[:, :sinks] += n * U * np.abs(arrays[7].astype(np.float64)).sum(0)
     return [dq, delta] if by_query else [dk, dv]
 
 

@@ -72,6 +72,24 @@ def test_attention_gradients(hip_backend_session, case):
         check(hip_backend_session, kernel, arrays, cases.attention_grad_bounds)
 
 
+@pytest.mark.parametrize("pieces", [1, 3, 64])
+@pytest.mark.parametrize("case", [c for c in cases.ATTENTIONS if c[6] and c[7] and 60 <= c[2] <= 300], ids=str)
+def test_attention_gradients_of_sinks(hip_backend_session, case, pieces):
+    """The rows past a tile's window, summed in pieces, and the key gradient that takes the pieces."""
+    (_, _), (whole, whole_arrays), (far, arrays), (joined, joined_arrays) = cases.attention_grad_cases(*case, np.random.default_rng(18), pieces)
+    want = ref.evaluate(far, cases.flat(arrays))
+    got = launch(hip_backend_session, far, arrays)
+    for g, w, b in zip(got, want, cases.attention_grad_bounds(far, arrays, want)):
+        assert (np.abs(g.astype(np.float64).sum(0) - w.sum(0)) <= b[0] + pieces * cases.U * np.abs(w).sum(0)).all()
+    check(hip_backend_session, joined, joined_arrays, cases.attention_grad_bounds)
+    # together: what the kernel without pieces gives
+    tail = joined_arrays[8:]
+    both = launch(hip_backend_session, joined, joined_arrays[:6] + got + tail)
+    want = ref.evaluate(whole, cases.flat(whole_arrays))
+    for g, w, b in zip(both, want, cases.attention_grad_bounds(whole, whole_arrays, want)):
+        assert (np.abs(g - w) <= 2 * b + cases.U * np.abs(w)).all()
+
+
 @pytest.mark.parametrize("splits", [2, 5, 64])
 @pytest.mark.parametrize("case", [c for c in cases.ATTENTIONS if c[1] <= 17], ids=str)
 def test_attention_in_pieces(hip_backend_session, case, splits):

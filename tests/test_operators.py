@@ -325,7 +325,11 @@ def test_malformed_operator_descriptors_are_rejected_with_a_message():
         att((0, 0, 0, 1), (q, k, _view((2, 5, 8, 2), mapping=((0, 1), (1, 1), (3, 1), (2, 1)), out=(2, 5, 2, 8)))),
         att((0, 0, 0, 1), (q, k, k), scale=float("nan")),
         OperatorKernel(OperatorSpec("AttentionGradQuery", (0, 0, 0), (1.0,)), (q, k, k, q, q, ident(2, 5, 3)), (0,)),
-        OperatorKernel(OperatorSpec("AttentionGradKeyValue", (0, 0, 0), (1.0,)), (q, k, k, k, ident(2, 5, 4), ident(2, 5, 4)), (0,)),
+        OperatorKernel(OperatorSpec("AttentionGradKeyValue", (0, 0, 0, 0), (1.0,)), (q, k, k, k, ident(2, 5, 4), ident(2, 5, 4)), (0,)),
+        OperatorKernel(OperatorSpec("AttentionGradKeyValue", (3, 2, 0, 2), (1.0,)), (q, k, k, q, ident(2, 5, 4), ident(2, 5, 4)), (0,)),
+        OperatorKernel(OperatorSpec("AttentionGradKeyValue", (3, 2, 0, 2), (1.0,)), (q, k, k, q, ident(2, 5, 4), ident(2, 5, 4)) + (ident(3, 2, 2, 2, 8),) * 2, (0,)),
+        OperatorKernel(OperatorSpec("AttentionGradSinks", (3, 2, 0, 65), (1.0,)), (q, k, k, q, ident(2, 5, 4), ident(2, 5, 4)), (0, 1)),
+        OperatorKernel(OperatorSpec("AttentionGradSinks", (0, 2, 0, 2), (1.0,)), (q, k, k, q, ident(2, 5, 4), ident(2, 5, 4)), (0, 1)),
         OperatorKernel(OperatorSpec("AttentionJoin"), (ident(3, 2, 5, 4, 8), ident(2, 2, 5, 4)), (0,)),
         OperatorKernel(OperatorSpec("DualMatMul", (DUAL_GATED, 4, 1)), (ident(3, 4), ident(4, 5), ident(4, 5)), (0,)),
         OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0, 1)), (ident(3, 4), ident(5, 5), ident(5, 5)), (0,)),
@@ -374,7 +378,7 @@ def _compiled_kernels():
     out += [cases.rotary_case(*c, rng)[0] for c in cases.ROTARIES]
     out += [cases.attention_case(*c, rng)[0] for c in cases.ATTENTIONS]
     for c in cases.ATTENTIONS[:6]:
-        out += [k for k, _ in cases.attention_grad_cases(*c, rng)]
+        out += [k for k, _ in cases.attention_grad_cases(*c, rng, pieces=2 if c[6] and c[7] else 0)]
     out += [cases.dual_case(*c, rng)[0] for c in cases.DUALS if c[1] < 2000]
     out += [cases.gated_grad_case((5, 3), a, rng)[0] for a in range(4)]
     out += [cases.join_case(3, 2, 1, 2, 8, rng)[0]]
