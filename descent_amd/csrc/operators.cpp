@@ -448,7 +448,7 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
         return assemble(fk, def, kAttentionSource, "dsc_attention_grad_query" + size, "attention_grad_query",
                         {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), input_arg(fk, 3), input_arg(fk, 4), input_arg(fk, 5), start, length,
                          result_arg(fk, 0), result_arg(fk, 1)},
-                        q[0] * k[2] * up(rows, 64), 256, waves, g);
+                        q[0] * k[2] * up(rows, 64), 256, dp <= 64 ? 3 : waves, g);
     }
     if (sinks) {
         def.set("AT_GRAD_SINKS", 1);
