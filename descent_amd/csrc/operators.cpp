@@ -437,10 +437,13 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
         // few rows: no tile of keys is read twice, so each wave streams its own
         const bool few = op[3] > 1 || rows <= 64, split = !few && dim <= 128;
         def.set(few ? "AT_FEW_ROWS" : split ? "AT_FORWARD_SPLIT" : "AT_FORWARD", 1);
-        g->note = few ? "rows x16, keys in " + to_string(op[3]) + " pieces" : string(split ? "bf16x6 tiles 128x32" : "tiles 64x64");
+        // waves that share a tile of keys: eight, if their 256 rows still leave every CU a workgroup
+        const int row_waves = q[0] * k[2] * up(rows, 256) >= 256 ? 8 : 4;
+        def.set("AT_WAVES", row_waves);
+        g->note = few ? "rows x16, keys in " + to_string(op[3]) + " pieces" : split ? "bf16x6 tiles " + to_string(32 * row_waves) + "x32" : string("tiles 64x64");
         return assemble(fk, def, kAttentionSource, (few ? "dsc_attention_few" : "dsc_attention") + size, few ? "attention_few" : split ? "attention_split" : "attention",
                         {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), start, length, result_arg(fk, 0), result_arg(fk, 1)},
-                        q[0] * k[2] * (few ? up(rows, 16) * op[3] : up(rows, split ? 128 : 64)), 256, waves, g);
+                        q[0] * k[2] * (few ? up(rows, 16) * op[3] : up(rows, split ? 32 * row_waves : 64)), split ? 64 * row_waves : 256, waves, g);
     }
     g->note = "tiles 64x64";
     if (grad_q) {
