@@ -520,7 +520,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
         def.set("DM_FEW_VEC", b_rows && n % 4 == 0 ? 1 : 0);
         args.erase(args.begin() + 1);
         g->note = "columns x32, k in 128 slices";
-        return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_few" + size, "gated_few_rows", args, up(n, 32), 1024, 1, g);
+        return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_few" + size, "gated_few_rows", args, up(n, 32), 1024, 4, g);
     }
     // Tile.  A CU's step of 16 k costs 2.4 us with 256x256 (8 waves of 128x64), 0.73 with 128x128 (8 waves of 32x64; with 4
     // waves of 64x64 0.83) and, alone on its CU, 0.55 with 64x64: the largest tile that leaves no CU without one, and
