@@ -24,6 +24,7 @@ from .operators import (
     DUAL_GATED,
     DUAL_SUM,
     OperatorSpec,
+    append_spec,
     attention_ints,
     attention_splits,
     dual_matmul_shapes,
@@ -452,6 +453,13 @@ class Array:
         k, v = self._lift(k), self._lift(v)
         start, length = (None if a is None else self._lift(a) for a in (start, length))
         return self._attention(k, v, window, sinks, scale, start, length)[0]
+
+    def cache_append(self, rows, start) -> "Array":
+        """self, [batch, capacity, width], with rows [batch, tokens, width] in place of its rows from start[b] on (u32
+        [batch]); rows past the capacity are dropped.  The buffer is updated in place, as by scatter_add: nothing else
+        may read the old values."""
+        rows, start = self._lift(rows), self._lift(start)
+        return emit([self, rows, start], append_spec(self.shape, rows.shape, start.shape), 1)[0]
 
     def gated_dense(self, w_gate, w_up, activation: str = "silu") -> "Array":
         """activation(self w_gate) * (self w_up) for [rows, width] and two [width, hidden] weights: both products, the

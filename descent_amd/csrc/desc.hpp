@@ -179,7 +179,7 @@ int64_t reference_group_count(const dsc_kernel_desc& d);
 std::string label_name(const dsc_kernel_desc& d);
 
 // Sequence-model operators (operators.cpp): kinds from DSC_KERNEL_RMS_NORM on.
-inline bool is_operator(int kind) { return kind >= DSC_KERNEL_RMS_NORM && kind <= DSC_KERNEL_ATTENTION_GRAD_SINKS; }
+inline bool is_operator(int kind) { return kind >= DSC_KERNEL_RMS_NORM && kind <= DSC_KERNEL_CACHE_APPEND; }
 std::string validate_operator(const dsc_kernel_desc& d);
 // All results of a valid operator descriptor, whether it writes them or not.
 std::vector<dsc_shape> operator_results(const dsc_kernel_desc& d);

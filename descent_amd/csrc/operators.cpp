@@ -13,7 +13,7 @@ using std::string;
 using std::to_string;
 
 const char* const kNames[] = {"RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionJoin", "AttentionGradQuery", "AttentionGradKeyValue",
-                              "DualMatMul", "GatedGrad", "AttentionGradSinks"};
+                              "DualMatMul", "GatedGrad", "AttentionGradSinks", "CacheAppend"};
 
 float as_float(uint32_t bits) {
     float f;
@@ -95,6 +95,7 @@ std::vector<dsc_shape> operator_results(const dsc_kernel_desc& d) {
         return {out, out};
     }
     case DSC_KERNEL_GATED_GRAD: return {in[0].out_shape, in[0].out_shape};
+    case DSC_KERNEL_CACHE_APPEND: return {shape_of({in[0].out_shape.dims[0], d.op_int[0], in[0].out_shape.dims[2]})};
     default: return {};
     }
 }
@@ -217,6 +218,12 @@ string validate_operator(const dsc_kernel_desc& d) {
         if (op[0] < 0 || op[0] > 3 || d.n_inputs != 3) return name + "unknown activation or wrong number of operands";
         if (!same_shape(in[0].out_shape, in[1].out_shape) || !same_shape(in[0].out_shape, in[2].out_shape)) return name + "operands differ in shape";
         e = views({}, false);
+        break;
+    }
+    case DSC_KERNEL_CACHE_APPEND: {
+        if (d.n_inputs != 2 || !ranks({3, 1}) || dims(1)[0] != dims(0)[0]) return name + "takes rows and a start per sequence";
+        if (op[0] < 1) return name + "capacity must be positive";
+        e = views({0}, false);
         break;
     }
     default: return "unknown kernel kind";
@@ -346,6 +353,7 @@ string gen_rotary(const FusedKernel& fk, Generated* g) {
     int64_t each = std::min(heads, std::max<int64_t>(1, 1024 / units));
     while (each > 1 && up(tokens, tok) * up(heads, each) < 512 && tok * each * units > 256) each = up(each, 2);
     Defines def;
+    def.set("RO_ROTARY", 1);
     def.set64("RO_TOKENS", tokens);
     def.set64("RO_T", x[1]);
     def.set("RO_HEADS", heads);
@@ -368,6 +376,27 @@ string gen_rotary(const FusedKernel& fk, Generated* g) {
     return assemble(fk, def, kRotarySource, "dsc_rotary_n" + to_string((long long)element_count(d.shape)), "rotary",
                     {input_arg(fk, 0), input_arg(fk, 1), d.op_int[2] ? input_arg(fk, 2, true) : "(const uint*)nullptr", result_arg(fk, 0)},
                     up(tokens, tok) * up(heads, each), 256, 1, g);
+}
+
+string gen_cache_append(const FusedKernel& fk, Generated* g) {
+    const dsc_kernel_desc& d = fk.main.raw();
+    const int64_t* x = d.inputs[0].out_shape.dims;
+    const Operand o(d.inputs[0]);
+    const int vec = x[2] % 4 == 0 && o.quads(d.inputs[0], 2) ? 4 : 1;
+    const int64_t units = x[0] * x[1] * (x[2] / vec);
+    Defines def;
+    def.set64("CA_UNITS", units);
+    def.set64("CA_TOKENS", x[1]);
+    def.set64("CA_CAPACITY", d.op_int[0]);
+    def.set64("CA_WIDTH", x[2]);
+    def.set("CA_VEC", vec);
+    def.set64("CA_BASE", o.base);
+    def.set64("CA_SB", o.stride[0]);
+    def.set64("CA_ST", o.stride[1]);
+    g->note = "x" + to_string(vec);
+    g->algo_bytes = 8.0 * (double)(x[0] * x[1]) * (double)x[2];
+    return assemble(fk, def, kRotarySource, "dsc_cache_append_n" + to_string((long long)(x[0] * x[1] * x[2])), "cache_append",
+                    {input_arg(fk, 0), input_arg(fk, 1, true), result_arg(fk, 0)}, up(units, 256), 256, 1, g);
 }
 
 string gen_attention(const FusedKernel& fk, Generated* g) {
@@ -562,6 +591,7 @@ string generate_operator(const FusedKernel& fk, Generated* out) {
     case DSC_KERNEL_RMS_NORM:
     case DSC_KERNEL_RMS_NORM_GRAD: return gen_rms_norm(fk, out);
     case DSC_KERNEL_ROTARY: return gen_rotary(fk, out);
+    case DSC_KERNEL_CACHE_APPEND: return gen_cache_append(fk, out);
     case DSC_KERNEL_DUAL_MATMUL:
     case DSC_KERNEL_GATED_GRAD: return gen_dual_matmul(fk, out);
     default: return gen_attention(fk, out);

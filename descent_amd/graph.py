@@ -580,12 +580,15 @@ class Graph:
                     [ClusterOutput(nid, copy_from=acc.node_id)],
                 )
             elif op.kind == "Operator":
+                in_place = None
+                if op.a.name == "CacheAppend":  # operand 0 becomes the result
+                    in_place, src = src[0].node_id, src[1:]
                 results = {ops.nodes[s].op.a: s for s in ops.successors(nid) if ops.nodes[s].op.kind == "Result"}
                 kept = sorted(results)
                 cluster = Cluster(
                     OperatorKernel(op.a, tuple(s.view for s in src), (0, *kept)),
                     [s.node_id for s in src],
-                    [ClusterOutput(nid)] + [ClusterOutput(results[i]) for i in kept],
+                    [ClusterOutput(nid, copy_from=in_place)] + [ClusterOutput(results[i]) for i in kept],
                 )
                 for i in kept:
                     ops.nodes[results[i]].cluster_id = next_cluster

@@ -202,32 +202,25 @@ class GatedFeedForward(Module):
 
 
 class KeyValueCache:
-    """Rotated keys and values of `batch` sequences of up to `capacity` tokens, as SelfAttention.step keeps them.  A slot is
-    zero until its token is written; `reset` empties the cache for new sequences."""
+    """Rotated keys and values of `batch` sequences of up to `capacity` tokens, as SelfAttention.step keeps them."""
 
     def __init__(self, env, batch: int, capacity: int, groups: int, head_dim: int):
-        self.batch, self.capacity, self.groups, self.head_dim = batch, capacity, groups, head_dim
-        self.keys = env.static_parameter([batch * capacity, groups * head_dim], "keys")
-        self.values = env.static_parameter([batch * capacity, groups * head_dim], "values")
-        self.reset(env)
-
-    def reset(self, env) -> None:
+        self.shape = [batch, capacity, groups, head_dim]
+        self.keys = env.static_parameter(self.shape, "keys")
+        self.values = env.static_parameter(self.shape, "values")
         for p in (self.keys, self.values):
             env.writer(p).zero_fill()
 
     def append(self, scope, parameter: Parameter, new: Array, start: Array) -> Array:
-        """Writes new [batch, tokens, groups, dim] behind the `start` tokens that each sequence holds, in place (a
-        ScatterAdd onto zeros), and returns the whole array.  Tokens past the capacity are dropped."""
-        batch, tokens, groups, dim = new.shape
-        if [batch, groups, dim] != [self.batch, self.groups, self.head_dim]:
-            raise ValueError(f"cache holds [{self.batch}, {self.capacity}, {self.groups}, {self.head_dim}], got {new.shape!r}")
-        place = start.reshape([batch, 1]) + scope.coord(tokens).value().into_u32()
-        row = scope.coord(batch).value().into_u32().reshape([batch, 1]) * self.capacity + place
-        # (an index past the array is dropped; this one is, whatever the array)
-        row = place.into_f32().select_gt(float(self.capacity - 1), scope.literal_u32(0x7F000000), row).reshape([batch * tokens])
-        whole = scope.parameter_value(parameter).scatter_add(new.reshape([batch * tokens, groups * dim]), 0, row)
+        """Writes new [batch, tokens, groups, dim] behind the `start` tokens that each sequence holds, in place, and
+        returns the whole array.  Tokens past the capacity are dropped."""
+        batch, capacity, groups, dim = self.shape
+        if [new.shape[0], new.shape[2], new.shape[3]] != [batch, groups, dim]:
+            raise ValueError(f"cache holds {parameter.shape!r}, got {new.shape!r}")
+        old = scope.parameter_value(parameter).reshape([batch, capacity, groups * dim])
+        whole = old.cache_append(new.reshape([batch, new.shape[1], groups * dim]), start).reshape(self.shape)
         scope.write_parameter_value(parameter, whole)
-        return whole.reshape([self.batch, self.capacity, groups, dim])
+        return whole
 
 
 class SelfAttention(Module):

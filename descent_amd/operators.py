@@ -18,7 +18,7 @@ from .shape import Shape, View
 # kinds, in the order of dsc_kernel_kind from DSC_KERNEL_RMS_NORM on
 OPERATORS = (
     "RmsNorm", "RmsNormGrad", "Rotary", "Attention", "AttentionJoin", "AttentionGradQuery", "AttentionGradKeyValue",
-    "DualMatMul", "GatedGrad", "AttentionGradSinks",
+    "DualMatMul", "GatedGrad", "AttentionGradSinks", "CacheAppend",
 )
 ACTIVATIONS = ("silu", "gelu", "relu", "sigmoid")
 LAYOUTS = ("half", "interleaved")
@@ -39,6 +39,7 @@ class OperatorSpec:
     AttentionGradSinks, AttentionGradKeyValue   the same and pieces
     DualMatMul             ints (mode, activation, splits)
     GatedGrad              ints (activation,)
+    CacheAppend            ints (capacity,); the node's operand 0 is the cache, taken over in place
     """
 
     name: str
@@ -78,6 +79,8 @@ class OperatorSpec:
             mode, _, splits = self.ints
             out = Shape(((splits,) if splits > 1 else ()) + (shapes[0][0], shapes[-1][1]))
             return {DUAL_GATED: [out] * 3, DUAL_SUM: [out], DUAL_BOTH: [out] * 2}[mode]
+        if name == "CacheAppend":
+            return [Shape((shapes[-2][0], self.ints[0], shapes[-2][2]))]
         assert name == "GatedGrad"
         return [shapes[0], shapes[0]]
 
@@ -89,6 +92,8 @@ class OperatorSpec:
             return "matrix"
         if name == "Rotary":
             return "rows" if arg == 0 else "dense"
+        if name == "CacheAppend":
+            return "rows" if arg == 1 else "dense"
         if name == "Attention":
             return "rows" if arg < 3 else "dense"
         if name == "AttentionGradQuery":
@@ -231,6 +236,13 @@ def attention_ints(q: Shape, k: Shape, v: Shape, window, sinks: int, start, leng
     _need(start is not None or q[1] <= k[1], f"attention: {q[1]} queries behind {k[1]} keys need `start`")
     has = (1 if start is not None else 0) | (2 if length is not None else 0)
     return (window or 0, min(sinks, k[1]) if window else 0, has)
+
+
+def append_spec(cache: Shape, rows: Shape, start: Shape) -> OperatorSpec:
+    _need(len(cache) == 3 and len(rows) == 3 and rows[0] == cache[0] and rows[2] == cache[2],
+          f"cache_append: rows {rows!r} do not fit the cache {cache!r}")
+    _need(tuple(start) == (cache[0],), f"cache_append: start must be [{cache[0]}], got {start!r}")
+    return OperatorSpec("CacheAppend", (cache[1],))
 
 
 def attention_splits(q: Shape, k: Shape, window, sinks: int) -> int:

@@ -88,7 +88,8 @@ typedef enum dsc_kernel_kind {
     DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE = 13,
     DSC_KERNEL_DUAL_MATMUL = 14,
     DSC_KERNEL_GATED_GRAD = 15,
-    DSC_KERNEL_ATTENTION_GRAD_SINKS = 16
+    DSC_KERNEL_ATTENTION_GRAD_SINKS = 16,
+    DSC_KERNEL_CACHE_APPEND = 17
 } dsc_kernel_kind;
 
 /* kernel.rs:8-35 `PerElementKernelOp` variants */
@@ -175,6 +176,9 @@ typedef struct dsc_pe_op {
  *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (those two), (start), (length)
  *                  op_int {window, sinks, as above, pieces or 0: the two are not given and nothing is left out}
  *                  out 0: dk; 1: dv
+ *   CACHE_APPEND   in  rows [batch,tokens,width] (s), start [batch]     op_int {capacity}
+ *                  out 0 (in/out, as SCATTER_ADD's accumulator): [batch,capacity,width]; row t of sequence b replaces the
+ *                  cache's row start[b] + t, rows past the capacity are dropped
  *   DUAL_MATMUL    op_int {dsc_dual_mode, dsc_activation, splits}; with splits > 1 (SUM and BOTH) the k range is cut into
  *                  that many pieces and the results have a leading axis of that extent, to be summed over
  *                  GATED in a [m,k], b0, b1 [k,n] (s)        out 0: act(a b0) * (a b1) [m,n]; 1: a b0; 2: a b1

@@ -89,6 +89,9 @@ class CpuBackend:
         self.launches.append(kernel.label_name())
         if isinstance(kernel, OperatorKernel):
             n = len(kernel.inputs)
+            if kernel.spec.name == "CacheAppend":
+                operators.append(kernel, *handles)
+                return
             for handle, value in zip(handles[n:], operators.evaluate(kernel, handles[:n])):
                 handle[:] = value.astype(np.float32).ravel()
             return

@@ -123,6 +123,17 @@ def activation(name, g):
     return (s, s * (1.0 - s)) if name == "sigmoid" else (g * s, s * (1.0 + g * (1.0 - s)))
 
 
+def append(kernel, rows, start, cache):
+    """CacheAppend on the cache's own buffer."""
+    rows = through(kernel.inputs[0], rows)
+    at = np.ascontiguousarray(through(kernel.inputs[1], start)).view(np.uint32)
+    whole = cache[: kernel.shape.element_count()].reshape(tuple(kernel.shape))
+    for b in range(rows.shape[0]):
+        for t in range(rows.shape[1]):
+            if int(at[b]) + t < whole.shape[1]:
+                whole[b, int(at[b]) + t] = rows[b, t]
+
+
 def evaluate(kernel, arrays):
     """The kernel's results, in 64 bits, in the order in which it binds them."""
     spec, ints, floats = kernel.spec, kernel.spec.ints, kernel.spec.floats

@@ -43,6 +43,7 @@ pub const DSC_KERNEL_ATTENTION_GRAD_KEY_VALUE: i32 = 13;
 pub const DSC_KERNEL_DUAL_MATMUL: i32 = 14;
 pub const DSC_KERNEL_GATED_GRAD: i32 = 15;
 pub const DSC_KERNEL_ATTENTION_GRAD_SINKS: i32 = 16;
+pub const DSC_KERNEL_CACHE_APPEND: i32 = 17;
 
 // dsc_pe_kind
 pub const DSC_PE_LOAD: i32 = 0;

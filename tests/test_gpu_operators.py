@@ -247,6 +247,34 @@ def test_strided_rotary_and_norm(hip_backend_session, case):
             assert rel_l2(g, w) <= 64 * cases.U
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1), (3, 2, 5, 8), (2, 7, 9, 130), (4, 1, 33, 64)], ids=str)
+def test_cache_append(hip_backend_session, shape):
+    """Rows replace what the cache holds; those past the capacity are dropped, the others untouched."""
+    batch, tokens, capacity, width = shape
+    rng = np.random.default_rng(19)
+    rows, cache = cases.normal(rng, batch, tokens, width), cases.normal(rng, batch, capacity, width)
+    start = rng.integers(0, capacity + 1, batch).astype(np.uint32)
+    start[0] = 0xFFFFFFFF if batch > 2 else 0
+    whole = rng.standard_normal((batch, tokens, width + 4)).astype(np.float32)
+    whole[:, :, 4:] = rows
+    dense = Shape(rows.shape).identity_view()
+    sliced = View(Shape(whole.shape), (0, 0, 4), dense.mapping, dense.output_shape)
+    be = hip_backend_session
+    for array, view in ((rows, dense), (whole, sliced)):
+        kernel = OperatorKernel(OperatorSpec("CacheAppend", (capacity,)), (view, Shape((batch,)).identity_view()), (0,))
+        handles = []
+        for a in cases.flat([array, start, cache]):
+            handles.append(be.alloc(a.nbytes))
+            be.write(handles[-1], 0, a)
+        be.launch(kernel, handles, 0)
+        got = np.frombuffer(be.read(handles[2], 0, cache.nbytes), np.float32)
+        want = cache.reshape(-1).copy()
+        ref.append(kernel, *cases.flat([array, start]), want)
+        assert np.array_equal(got, want)
+        for h in handles:
+            be.free(h)
+
+
 @pytest.mark.parametrize("tokens,keys", [(70, 70), (1, 300), (3, 90)])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
 def test_masked_elements_take_no_part(hip_backend_session, tokens, keys, value):
@@ -397,12 +425,40 @@ def test_block_serves_what_it_computes_whole(hip_backend_session):
         assert rel_l2(env.read_parameter(yt), whole[:, done : done + n]) <= 1e-5
         done += n
     assert done == tokens
+    # the last five tokens once more: their slots are written again, the answer is the same
+    again = graphs[5][2]
+    last = env.read_parameter(again)
+    env.run(graphs[5][0], 0)
+    assert np.array_equal(env.read_parameter(again), last)
     # past the capacity nothing is written
     keys = env.read_parameter(cache.keys)
     graph, xt, yt = graphs[5]
     env.write_parameter(start, np.full(batch, tokens + 2, np.uint32))
     env.run(graph, 0)
     assert np.array_equal(env.read_parameter(cache.keys), keys)
+
+
+def test_block_without_device_allocation(hip_backend_session):
+    """run_static: intermediates in the library's scratch array, written parameters alternating with a spare buffer."""
+    from descent_amd import Environment
+
+    results = []
+    for static in (False, True):
+        env = Environment(hip_backend_session)
+        rng = np.random.default_rng(20)
+        block, _ = _block(env, rng)
+        data = rng.standard_normal((2, 3, 48)).astype(np.float32)
+        x, y = env.static_parameter_with_data(data.shape, "x", data), env.static_parameter(data.shape, "y")
+        env.writer(y).zero_fill()
+        start = env.static_parameter([2], "start")
+        cache = block.attention.cache(env, 2, 20)
+        graph = env.build_graph(lambda s: s.write_parameter_value(y, block.step(s.parameter_value(x), cache, s.parameter_value(start).to_u32_bits())))
+        for done in (0, 3, 6):
+            env.write_parameter(start, np.full(2, done, np.uint32))
+            (env.run_static if static else env.run)(graph, 0)
+        results.append([env.read_parameter(p) for p in (y, cache.keys, cache.values)])
+    for a, b in zip(*results):
+        assert np.isfinite(a).all() and np.array_equal(a, b)
 
 
 def test_two_environments_at_once(hip_backend_session):

@@ -287,6 +287,10 @@ def test_arguments_are_checked():
         with pytest.raises(ValueError) as e:
             env.build_graph(f)
         assert len(str(e.value)) > 15, i
+    with pytest.raises(ValueError, match="do not fit"):
+        env.build_graph(lambda s: s.parameter_value(env.static_parameter([2, 9, 5], "c")).cache_append(s.parameter_value(env.static_parameter([2, 1, 6], "r")), s.parameter_value(t)))
+    with pytest.raises(ValueError, match="start must be"):
+        env.build_graph(lambda s: s.parameter_value(env.static_parameter([2, 9, 5], "c")).cache_append(s.parameter_value(env.static_parameter([2, 1, 5], "r")), s.parameter_value(t)))
     cache = SelfAttention(env, 8, 2).cache(env, 2, 4)
     with pytest.raises(ValueError, match="cache holds"):
         env.build_graph(lambda s: cache.append(s, cache.keys, s.parameter_value(q), s.parameter_value(t)))
@@ -335,6 +339,8 @@ def test_malformed_operator_descriptors_are_rejected_with_a_message():
         OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0, 1)), (ident(3, 4), ident(5, 5), ident(5, 5)), (0,)),
         OperatorKernel(OperatorSpec("DualMatMul", (DUAL_SUM, 0, 1)), (ident(3, 4), ident(2, 4), ident(4, 5), ident(4, 5)), (0,)),
         OperatorKernel(OperatorSpec("DualMatMul", (DUAL_BOTH, 0, 1)), (_view((6, 8), mapping=((0, 2), (1, 2)), out=(3, 4)), ident(4, 5), ident(4, 5)), (0,)),
+        OperatorKernel(OperatorSpec("CacheAppend", (9,)), (ident(2, 3, 4), ident(3)), (0,)),
+        OperatorKernel(OperatorSpec("CacheAppend", (9,)), (ident(2, 4, 3).transposed(), ident(2)), (0,)),
         OperatorKernel(OperatorSpec("GatedGrad", (4,)), (ident(3, 4),) * 3, (0,)),
         OperatorKernel(OperatorSpec("GatedGrad", (0,)), (ident(3, 4), ident(3, 4), ident(4, 3)), (0,)),
     ]
@@ -382,6 +388,7 @@ def _compiled_kernels():
     out += [cases.dual_case(*c, rng)[0] for c in cases.DUALS if c[1] < 2000]
     out += [cases.gated_grad_case((5, 3), a, rng)[0] for a in range(4)]
     out += [cases.join_case(3, 2, 1, 2, 8, rng)[0]]
+    out += [OperatorKernel(OperatorSpec("CacheAppend", (9,)), (Shape((2, 3, w)).identity_view(), Shape((2,)).identity_view()), (0,)) for w in (8, 7)]
     return out
 
 
