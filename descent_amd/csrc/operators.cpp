@@ -489,13 +489,21 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
                          result_arg(fk, 0), result_arg(fk, 1)},
                         q[0] * k[2] * up(std::min<int64_t>(op[1], k[1]), 16) * op[3], 256, waves, g);
     }
+    // Key gradient: four waves, two workgroups per CU, for heads of up to 64 (2048 tokens, 4 x 16 heads of 64: 697 us against
+    // 769 with eight); eight up to 128, where two of four waves hold 64 KB of tiles each (4096 tokens, 16 over 4 heads of 128,
+    // window 1024: 752 against 962); four beyond, one per SIMD.  Tiles of 32 keys while all of them run at once (2 x 512
+    // tokens, 8 heads of 64: 33 against 52; 4 heads of 128: 55 against 91), else of 64 (32 x 512 tokens: 201 against 234).
+    const int key_waves = dp > 64 && dp <= 128 ? 8 : 4;
+    const int keys = q[0] * k[2] * up(k[1], 64) <= (dp <= 64 ? 256 : 128) ? 32 : 64;
+    def.set("AT_KEYS", keys);
     def.set("AT_GRAD_KEY_VALUE", 1);
-    def.set("AT_HALVES", waves);
+    g->note = "tiles " + to_string(keys) + "x64, " + to_string(key_waves) + " waves";
+    def.set("AT_SHARES", 16 * key_waves / keys);
     return assemble(fk, def, kAttentionSource, "dsc_attention_grad_key_value" + size, "attention_grad_key_value",
                     {input_arg(fk, 0), input_arg(fk, 1), input_arg(fk, 2), input_arg(fk, 3), input_arg(fk, 4), input_arg(fk, 5),
                      joins ? input_arg(fk, 6) : "(const float*)nullptr", joins ? input_arg(fk, 7) : "(const float*)nullptr", start, length,
                      result_arg(fk, 0), result_arg(fk, 1)},
-                    q[0] * k[2] * up(k[1], 64), 256 * waves, waves, g);
+                    q[0] * k[2] * up(k[1], keys), 64 * key_waves, waves, g);
 }
 
 string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
