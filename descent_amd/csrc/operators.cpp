@@ -562,16 +562,18 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     // Tile.  A CU's step of 16 k costs 2.4 us with 256x256 (8 waves of 128x64), 0.73 with 128x128 (8 waves of 32x64; with 4
     // waves of 64x64 0.83) and, alone on its CU, 0.55 with 64x64: the largest tile that leaves no CU without one, and
     // the smallest where even that many do not fill the CUs (1001 x 1366 columns x 512 k of both products: 32 us with
-    // 128x128, 37 with 64x64; 1001 x 500, k 2 x 1366, not split: 113 and 98).
+    // 128x128, 37 with 64x64; 1001 x 500, k 2 x 1366, not split: 113 and 98).  Up to 64 rows there are too few tiles for the
+    // CUs and a step's latency counts: four groups of waves share k (16 x 4096 into 8000: 162 us with one group, 120 with
+    // two, 86 with four; 64 x 2048 into 1366: 83, 62, 46, and 66 with tiles of 64x64).
     struct Tile {
-        int bm, bn, wm, wn, ahead;
+        int bm, bn, wm, wn, ahead, groups;
     };
     const int64_t splits = d.op_int[2];
     auto count = [&](int bm, int bn) { return up(m, bm) * up(n, paired ? bn / 2 : bn) * splits; };
-    Tile t = {128, 128, 4, 2, 2};
-    if (m <= 32) t = {32, 128, 1, 2, 4};
-    else if (count(256, 256) >= 256) t = {256, 256, 2, 4, 2};
-    else if (count(64, 64) <= 256) t = {64, 64, 2, 1, 4};
+    Tile t = {128, 128, 4, 2, 2, 1};
+    if (m <= 64) t = {32, 128, 1, 2, 4, 4};
+    else if (count(256, 256) >= 256) t = {256, 256, 2, 4, 2, 1};
+    else if (count(64, 64) <= 256) t = {64, 64, 2, 1, 4, 1};
     const int64_t tiles_m = up(m, t.bm), tiles_n = up(n, paired ? t.bn / 2 : t.bn);
     if (tiles_m * tiles_n * splits >= (int64_t(1) << 30)) return "kernel too large: more than 2^30 tiles";
     def.set("DM_BM", t.bm);
@@ -580,6 +582,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     def.set("DM_WN", t.wn);
     def.set("DM_AHEAD", t.ahead);
     def.set("DM_SPLITS", splits);
+    def.set("DM_KGROUPS", t.groups);
     def.set("DM_A_KC", a_kc ? 1 : 0);
     def.set("DM_B_KC", b_kc ? 1 : 0);
     def.set("DM_A_VEC", a_vec && k % 4 == 0 ? 1 : 0);  // (quads that are moved back to end with k keep their alignment)
@@ -589,7 +592,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     def.set("DM_GROUP", 8);
     g->note = "bf16x6 32x32x16 tile " + to_string(t.bm) + "x" + to_string(t.bn) + "x16 waves " + to_string(t.wm) + "x" + to_string(t.wn) + " A" +
               (a_kc ? a_vec ? "k4" : "k1" : "r") + " B" + (b_kc ? b_vec ? "k4" : "k1" : "r");
-    return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_" + what + size, "dual_matmul", args, up(tiles_m * tiles_n * splits, 8) * 8, 64 * t.wm * t.wn, 2, g);
+    return assemble(fk, def, kDualMatmulSource, "dsc_dual_matmul_" + what + size, "dual_matmul", args, up(tiles_m * tiles_n * splits, 8) * 8, 64 * t.wm * t.wn * t.groups, 2, g);
 }
 
 }  // namespace
