@@ -1,0 +1,24 @@
+"""CPU: what the operators' kernels read and write stays inside their operands (host_kernel.py)."""
+import re
+
+import numpy as np
+import pytest
+
+import host_kernel
+import operator_cases as cases
+from descent_amd import hip_backend
+
+
+def _split_grid(kernel):
+    """Workgroups of the attention kernel for more than 64 rows of a key head and heads of up to 128."""
+    define = dict(re.findall(r"#define (AT_\w+) \(?(-?\d+)", hip_backend.codegen_source(kernel)))
+    assert "AT_FORWARD_SPLIT" in define
+    b, t, h, g, waves = (int(define["AT_" + n]) for n in ("B", "T", "H", "G", "WAVES"))
+    return b * g * -(-t * (h // g) // (32 * waves))
+
+
+@pytest.mark.parametrize("dim", [16, 48, 80, 112, 20, 32, 128, 15, 31])
+def test_prompt_attention_reads_inside_its_operands(dim):
+    """Heads that are no multiple of the 32 elements that a matrix instruction's tile takes end with the query row."""
+    kernel, arrays = cases.attention_case(2, 70, 70, 2, 2, dim, 20, 2, "none", np.random.default_rng(1))
+    host_kernel.run(kernel, arrays, _split_grid(kernel))
