@@ -4,7 +4,9 @@ import numpy as np
 import pytest
 
 import operator_cases as cases
+from descent_amd.operators import OperatorSpec
 from descent_amd.shape import Shape, View
+from oracle import operators as ref
 from test_gpu_operators import check, launch
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +30,118 @@ def test_query_rows_end_with_their_head(hip_backend_session, dim):
     for k, a in ((strided, [wide] + arrays[1:]), (kernel, padded)):
         for w, g in zip(want, launch(hip_backend_session, k, a)):
             assert np.array_equal(w, g)
+
+
+def _agree(got, want, bounds):
+    """NaN exactly where the definition has it, everything else within its bound."""
+    for i, (g, w, b) in enumerate(zip(got, want, bounds)):
+        assert np.array_equal(np.isnan(g), np.isnan(w)), f"result {i}: {np.isnan(g).sum()} NaN for {np.isnan(w).sum()}"
+        rest = ~np.isnan(w)
+        low = np.isneginf(w)
+        assert np.array_equal(np.isneginf(g), low), f"result {i}"
+        rest &= ~low
+        off = np.abs(g.astype(np.float64) - np.where(rest, w, 0.0))[rest] - (np.broadcast_to(b, w.shape) + cases.U * np.abs(w))[rest]
+        assert off.max(initial=-1.0) <= 0.0, f"result {i}: {off.max()}"
+
+
+def _clean(arrays):
+    return [np.where(np.isfinite(a), a, np.float32(0)) if a.dtype == np.float32 else a for a in arrays]
+
+
+def _forward(backend, kernel, arrays, splits):
+    """The kernel's results and the definition's, with the bounds of the same call without the odd elements."""
+    want = ref.evaluate(kernel, cases.flat(arrays))
+    bounds = cases.attention_bounds(kernel, _clean(arrays), ref.evaluate(kernel, cases.flat(_clean(arrays))))
+    if splits == 1:
+        return launch(backend, kernel, arrays), want, bounds
+    pieces = cases.kernel(OperatorSpec("Attention", kernel.spec.ints[:3] + (splits,), kernel.spec.floats), arrays)
+    part = launch(backend, pieces, arrays)
+    # the join's exponentials, sums and quotient, each against the largest value
+    largest = [np.abs(_clean(arrays)[2]).max(), 1.0]
+    joined = launch(backend, cases.kernel(OperatorSpec("AttentionJoin"), part), part)
+    return joined, want, [b + 8 * splits * cases.U * (np.where(np.isfinite(w), np.abs(w), 0.0) + m) for b, w, m in zip(bounds, want, largest)]
+
+
+# (batch, tokens, keys, heads, groups, dim, splits): a few rows, whole and in pieces; tiles in three parts; wide heads
+KERNELS = [(2, 1, 600, 4, 2, 64, 1), (2, 1, 600, 4, 2, 48, 2), (1, 3, 600, 2, 1, 200, 5), (1, 2, 600, 3, 3, 30, 64), (2, 70, 70, 4, 2, 64, 1),
+           (1, 80, 90, 2, 1, 48, 1), (1, 90, 90, 2, 2, 80, 1), (1, 70, 80, 1, 1, 31, 1), (1, 70, 70, 2, 1, 200, 1), (2, 80, 90, 2, 2, 160, 1)]
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("case", KERNELS, ids=str)
+def test_queries_that_are_not_finite(hip_backend_session, case, value):
+    """Every score of such a row is NaN or infinite, so the row is NaN, and so is its denominator; a row of padding is not."""
+    batch, tokens, keys, heads, groups, dim, splits = case
+    for window, sinks in ((0, 0), (20, 2), (1, 0)):
+        kernel, arrays = cases.attention_case(batch, tokens, keys, heads, groups, dim, window, sinks, "both", np.random.default_rng(22))
+        arrays[3][:] = [keys - tokens, 0][:batch]
+        arrays[4][:] = [keys, max(1, tokens - 4)][:batch]
+        arrays[0][:, :: max(1, tokens // 5), -1, dim // 2] = value  # the first row among them, which may see one key only
+        got, want, bounds = _forward(hip_backend_session, kernel, arrays, splits)
+        assert np.isnan(want[1]).any() and not np.isnan(want[1]).all()
+        _agree(got, want, bounds)
+
+
+@pytest.mark.parametrize("case", KERNELS, ids=str)
+def test_keys_that_are_not_numbers(hip_backend_session, case):
+    """A row is NaN if and only if it sees such a key: as one of many, as the only one of a row, of a block of 16 or of a
+    piece, as a sink, or its own new key behind a cache."""
+    batch, tokens, keys, heads, groups, dim, splits = case
+    for window, sinks, at in ((0, 0, 0), (0, 0, keys - tokens), (1, 0, keys - tokens), (1, 0, 16), (7, 3, 1), (0, 0, 16)):
+        kernel, arrays = cases.attention_case(batch, tokens, keys, heads, groups, dim, window, sinks, "both", np.random.default_rng(23))
+        arrays[3][:] = [16 if at == 16 and tokens < 16 else keys - tokens, 0][:batch]
+        arrays[4][:] = [keys, keys - 3][:batch]
+        arrays[1][:, at, :, dim - 1] = np.nan
+        got, want, bounds = _forward(hip_backend_session, kernel, arrays, splits)
+        assert np.isnan(want[0]).any()
+        _agree(got, want, bounds)
+
+
+@pytest.mark.parametrize("case", [c for c in KERNELS if c[1] > 60 or c[6] == 1], ids=str)
+def test_gradients_of_rows_that_are_not_numbers(hip_backend_session, case):
+    """A row whose query is NaN: its own gradient is NaN, and that of every key that it sees, and no other."""
+    batch, tokens, keys, heads, groups, dim, _ = case
+    for window, sinks in ((0, 0), (20, 2), (1, 0)):
+        (by_query, qa), (by_key, ka) = cases.attention_grad_cases(batch, tokens, keys, heads, groups, dim, window, sinks, "both", np.random.default_rng(24))
+        clean = [[a.copy() for a in arrays] for arrays in (qa, ka)]
+        start, length = qa[-2:]
+        row = next(t for t in range(tokens) if int(start[0]) + t < int(length[0]))
+        for arrays, touched in ((qa, (0, 3, 5)), (ka, (0, 4, 5))):
+            for i in touched:
+                arrays[i][0, row, 0] = np.nan  # the query, and what the forward pass made of it
+        for (k, arrays), without in zip(((by_query, qa), (by_key, ka)), clean):
+            bounds = cases.attention_grad_bounds(k, without, ref.evaluate(k, cases.flat(without)))
+            want = ref.evaluate(k, cases.flat(arrays))
+            assert np.isnan(want[0]).any() and np.isnan(want[1]).any()
+            _agree(launch(hip_backend_session, k, arrays), want, bounds)
+
+
+@pytest.mark.parametrize("tokens,keys,dim", [(1, 2000, 64), (70, 70, 48), (66, 66, 136)])
+def test_a_graph_passes_what_is_not_a_number_on(hip_backend_session, tokens, keys, dim):
+    """Through the public calls, forward and backward: a NaN query reaches its row and the gradients, a NaN key its readers."""
+    from descent_amd import Environment
+
+    rng = np.random.default_rng(25)
+    env = Environment(hip_backend_session)
+    data = {"q": cases.normal(rng, 1, tokens, 4, dim), "k": cases.normal(rng, 1, keys, 2, dim), "v": cases.normal(rng, 1, keys, 2, dim),
+            "dy": cases.normal(rng, 1, tokens, 4, dim)}
+    data["q"][0, 0, 1, 3] = np.nan
+    p = {n: env.static_parameter_with_data(a.shape, n, a) for n, a in data.items()}
+    out = {n: env.static_parameter(data[n if n != "y" else "q"].shape, n) for n in ("y", "q", "k", "v")}
+
+    def build(s):
+        y = s.parameter(p["q"]).attention(s.parameter(p["k"]), s.parameter(p["v"]))
+        y.loss_grad().accumulate(s.parameter_value(p["dy"]))
+        s.write_parameter_value(out["y"], y.value())
+        for n in "qkv":
+            s.write_parameter_value(out[n], s.parameter(p[n]).loss_grad())
+
+    graph = env.build_graph(build)
+    env.run(graph, 0)
+    got = {n: np.isnan(env.read_parameter(a)) for n, a in out.items()}
+    row = np.zeros((1, tokens, 4, dim), bool)
+    row[0, 0, 1] = True
+    seen = np.zeros((1, keys, 2, dim), bool)
+    seen[0, : keys - tokens + 1, 0] = True
+    assert np.array_equal(got["y"], row) and np.array_equal(got["q"], row)
+    assert np.array_equal(got["k"], seen) and np.array_equal(got["v"], seen)
