@@ -101,7 +101,7 @@ def run(kernel, arrays, grid):
     if not os.path.exists(CLANG):
         pytest.skip("no clang++")
     source = hip_backend.codegen_source(kernel)
-    source = re.sub(r"asm volatile\((.|\n)*?\);", "", source)  # (other kernels' helpers in the common prelude)
+    source = re.sub(r"asm( volatile)?\((.|\n)*?\);", "", source)  # (other kernels' helpers in the common prelude)
     entry, parameters = re.search(r'extern "C" __global__ __launch_bounds__\([^)]*\) void (\w+)\(([^)]*)\)', source).groups()
     block = int(re.search(r'extern "C" __global__ __launch_bounds__\((\d+)', source).group(1))
     sizes = [a.nbytes for a in arrays] + [kernel.result_shapes()[i].buffer_size() for i in kernel.results]

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import operator_cases as cases
-from descent_amd.operators import OperatorSpec
+from descent_amd.operators import ACTIVATIONS, DUAL_BOTH, DUAL_GATED, DUAL_SUM, OperatorSpec
 from descent_amd.shape import Shape, View
 from oracle import operators as ref
 from test_gpu_operators import check, launch
@@ -145,3 +145,51 @@ def test_a_graph_passes_what_is_not_a_number_on(hip_backend_session, tokens, key
     seen[0, : keys - tokens + 1, 0] = True
     assert np.array_equal(got["y"], row) and np.array_equal(got["q"], row)
     assert np.array_equal(got["k"], seen) and np.array_equal(got["v"], seen)
+
+
+LARGEST = np.finfo(np.float32).max  # past what rounds to a finite bfloat16
+
+
+@pytest.mark.parametrize("transposed", [(), (1, 2), (0, 3)], ids=str)
+@pytest.mark.parametrize("rows", [4, 40, 300])
+@pytest.mark.parametrize("mode", [DUAL_GATED, DUAL_SUM, DUAL_BOTH])
+def test_dual_products_of_the_largest_numbers(hip_backend_session, mode, rows, transposed):
+    """Elements of the largest magnitude beside small ones and zeros: the products are finite, and as good as all others."""
+    kernel, arrays = cases.dual_case(mode, rows, 70, 96, ACTIVATIONS.index("relu"), np.random.default_rng(26), transposed)
+    x = [a.T if i in transposed else a for i, a in enumerate(arrays)]
+    left = 2 if mode == DUAL_SUM else 1
+    for i, a in enumerate(x):
+        if i < left:
+            a[2, 5], a[1, 9] = LARGEST, -LARGEST
+            a[:, 50] *= np.float32(2.0 ** -80)
+            a[:, 51] = 0.0
+        else:
+            a[5], a[9] = a[5] * np.float32(2.0 ** -80), 0.0
+            a[50, 7], a[51, 8] = -LARGEST, LARGEST
+    check(hip_backend_session, kernel, arrays, cases.dual_bounds)
+
+
+@pytest.mark.parametrize("mode", [DUAL_GATED, DUAL_SUM, DUAL_BOTH])
+def test_dual_products_of_small_numbers(hip_backend_session, mode):
+    """Down to 2^-99 all three parts of a number are normal ones of the shorter type, and the bounds are the same."""
+    kernel, arrays = cases.dual_case(mode, 40, 70, 96, ACTIVATIONS.index("relu"), np.random.default_rng(27))
+    for i, a in enumerate(arrays):
+        left = i < (2 if mode == DUAL_SUM else 1)
+        a[:] = np.sign(a) * np.maximum(np.abs(a), 0.25) * np.float32(2.0 ** (-97 if left else 60))
+    check(hip_backend_session, kernel, arrays, cases.dual_bounds)
+
+
+@pytest.mark.parametrize("case", KERNELS, ids=str)
+def test_attention_to_the_largest_numbers(hip_backend_session, case):
+    """A key, a value and a query of the type's lowest value: harmless where the mask hides them or the other factor is 0,
+    and weighted like any other where a row sees them."""
+    batch, tokens, keys, heads, groups, dim, splits = case
+    for window, sinks in ((0, 0), (20, 2), (1, 0)):
+        kernel, arrays = cases.attention_case(batch, tokens, keys, heads, groups, dim, window, sinks, "both", np.random.default_rng(28))
+        arrays[3][:] = [keys - tokens, 0][:batch]
+        arrays[4][:] = [keys, max(1, tokens - 4)][:batch]
+        q, k, v = arrays[:3]
+        q[..., 0], k[:, [1, keys - tokens], :, 0] = 0.0, -LARGEST
+        k[..., dim - 1], q[:, tokens - 1, :, dim - 1] = 0.0, -LARGEST
+        v[:, keys - tokens, :, ::3] = -LARGEST
+        _agree(*_forward(hip_backend_session, kernel, arrays, splits))
