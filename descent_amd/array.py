@@ -747,7 +747,8 @@ class DualArray:
         return self._rms_norm(weight, epsilon, None)[0]
 
     def add_rms_norm(self, residual, weight, epsilon: float = 1e-6):
-        """(norm, sum): the gradients that arrive at both leave in one pass, and a sum that nothing reads costs nothing."""
+        """(norm, sum): the gradients that arrive at both leave in one pass, and one of them that no loss takes costs
+        nothing."""
         return self._rms_norm(weight, epsilon, residual)
 
     def rotary(self, frequencies, positions=None, layout: str = "half", magnitude: float = 1.0):

@@ -259,19 +259,37 @@ class Graph:
         assert len(self.ops_sorted) == len(self.ops.nodes), "op graph has a cycle"
 
     def _drop_absent_gradients(self):
-        """A norm's gradient takes the gradient of the sum that the norm left beside its result; where nothing read that
-        sum, the operand goes."""
+        """A norm's gradient takes the gradients of the norm and of the sum that the norm left beside it.  Where nothing
+        read that sum, the operand goes; where nothing read the norm, the sum's gradient is the whole answer and the
+        weight gets zeros."""
         ops = self.ops
-        for nid, node in ops.nodes.items():
-            if node.op.kind != "Operator" or node.op.a.name != "RmsNormGrad" or not node.op.a.ints[0]:
-                continue
-            eid = ops.arg_edge_ids(nid)[4]
+
+        def absent(eid):
             source = ops.edges[eid].src
             while ops.nodes[source].op == MOV and ops.in_edges(source):
                 source = ops.edges[ops.in_edges(source)[0]].src
-            if ops.nodes[source].op == MOV:
-                ops.remove_edge(eid)
+            return ops.nodes[source].op == MOV
+
+        for nid, node in list(ops.nodes.items()):
+            if node.op.kind != "Operator" or node.op.a.name != "RmsNormGrad" or not node.op.a.ints[0]:
+                continue
+            args = ops.arg_edge_ids(nid)
+            if absent(args[4]):
+                ops.remove_edge(args[4])
                 node.op = Op("Operator", OperatorSpec("RmsNormGrad", (0,) + node.op.a.ints[1:]))
+            elif absent(args[3]):
+                for share in [n for n in ops.successors(nid) if ops.nodes[n].op.kind == "Result"]:
+                    # (a Reduce over the weight's partial sums reads a buffer: its result is set to zeros instead)
+                    for zero in [share] + [n for n in ops.successors(share) if ops.nodes[n].op.kind == "Reduce"]:
+                        for eid in ops.in_edges(zero):
+                            ops.remove_edge(eid)
+                        literal = ops.new_node(node.colour, [1], Op("Literal", Literal.f32(0.0)))
+                        ops.nodes[zero].op = MOV
+                        ops.add_edge(literal, zero, 0, View.broadcast(Shape([1]), ops.nodes[zero].shape))
+                for eid in args[:4]:
+                    ops.remove_edge(eid)
+                ops.edges[args[4]].arg = 0
+                node.op = MOV
 
     def _eliminate_dead_code(self):
         """Keep what reaches an Output (src/graph.rs:150-165)."""
