@@ -432,7 +432,7 @@ string gen_attention(const FusedKernel& fk, Generated* g) {
     def.set("AT_D", dim);
     def.set("AT_DP", dp);
     def.set("AT_WINDOW", op[0]);
-    def.set("AT_SINKS", op[1]);
+    def.set("AT_SINKS", std::min<int64_t>(op[1], k[1]));  // (kernels round it up to tiles in 32 bits)
     def.set_float("AT_SCALE", as_float(d.op_float[0]));
     def.set("AT_START", op[2] & 1);
     def.set("AT_LENGTH", op[2] >> 1);

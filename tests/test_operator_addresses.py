@@ -7,6 +7,7 @@ import pytest
 import host_kernel
 import operator_cases as cases
 from descent_amd import hip_backend
+from descent_amd.operators import OperatorSpec
 
 
 def _split_grid(kernel):
@@ -22,3 +23,13 @@ def test_prompt_attention_reads_inside_its_operands(dim):
     """Heads that are no multiple of the 32 elements that a matrix instruction's tile takes end with the query row."""
     kernel, arrays = cases.attention_case(2, 70, 70, 2, 2, dim, 20, 2, "none", np.random.default_rng(1))
     host_kernel.run(kernel, arrays, _split_grid(kernel))
+
+
+@pytest.mark.parametrize("window", [20, 70])
+def test_more_sinks_than_keys(window):
+    """A descriptor may ask for any number of sinks: past the last key there are none, and nothing is read there."""
+    kernel, arrays = cases.attention_case(1, 90, 90, 2, 2, 32, window, 2, "none", np.random.default_rng(2))
+    most = cases.kernel(OperatorSpec("Attention", (window, 0x7FFFFFFF) + kernel.spec.ints[2:], kernel.spec.floats), arrays)
+    host_kernel.run(most, arrays, _split_grid(most))
+    all_of_them = cases.kernel(OperatorSpec("Attention", (window, 90) + kernel.spec.ints[2:], kernel.spec.floats), arrays)
+    assert hip_backend.codegen_source(most) == hip_backend.codegen_source(all_of_them)
