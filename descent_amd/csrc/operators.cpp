@@ -172,7 +172,8 @@ string validate_operator(const dsc_kernel_desc& d) {
         if (q[3] > 256) return name + "heads of more than 256 elements";
         if (op[0] < 0 || op[1] < 0) return name + "negative window or sinks";
         if (!(op[2] & 1) && q[1] > k[1]) return name + "more queries than keys need starts";
-        if (q[1] * (q[2] / k[2]) >= (int64_t(1) << 31)) return name + "kernel too large: rows of a key head";
+        // (kernels count rows in 32 bits and round them up to tiles of up to 256)
+        if (q[1] * (q[2] / k[2]) > (int64_t(1) << 31) - 512) return name + "kernel too large: rows of a key head";
         for (int i = arrays; i < d.n_inputs; ++i)
             if (!is_shape(in[i].out_shape, {q[0]})) return name + "starts and lengths must be [batch]";
         if (d.kind == DSC_KERNEL_ATTENTION) {

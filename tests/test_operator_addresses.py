@@ -7,7 +7,8 @@ import pytest
 import host_kernel
 import operator_cases as cases
 from descent_amd import hip_backend
-from descent_amd.operators import OperatorSpec
+from descent_amd.operators import OperatorKernel, OperatorSpec
+from descent_amd.shape import Shape
 
 
 def _split_grid(kernel):
@@ -33,3 +34,14 @@ def test_more_sinks_than_keys(window):
     host_kernel.run(most, arrays, _split_grid(most))
     all_of_them = cases.kernel(OperatorSpec("Attention", (window, 90) + kernel.spec.ints[2:], kernel.spec.floats), arrays)
     assert hip_backend.codegen_source(most) == hip_backend.codegen_source(all_of_them)
+
+
+def test_rows_of_a_key_head_are_counted_in_32_bits():
+    """Up to what a kernel adds to the last of them while it rounds up to tiles."""
+    def prompt(tokens):
+        q, k = Shape((1, tokens, 2, 4)).identity_view(), Shape((1, (1 << 30) - 1, 1, 4)).identity_view()
+        return OperatorKernel(OperatorSpec("Attention", (8, 0, 0, 1), (1.0,)), (q, k, k), (0, 1))
+
+    assert "attention_split" in hip_backend.codegen_source(prompt((1 << 30) - 300))
+    with pytest.raises(hip_backend.DescentHipError, match="rows of a key head"):
+        hip_backend.codegen_source(prompt((1 << 30) - 1))
