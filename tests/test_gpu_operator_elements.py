@@ -193,3 +193,12 @@ def test_attention_to_the_largest_numbers(hip_backend_session, case):
         k[..., dim - 1], q[:, tokens - 1, :, dim - 1] = 0.0, -LARGEST
         v[:, keys - tokens, :, ::3] = -LARGEST
         _agree(*_forward(hip_backend_session, kernel, arrays, splits))
+
+
+@pytest.mark.parametrize("width", [8196, 16384, 20001, 32768, 32772, 65536])
+def test_wide_norms(hip_backend_session, width):
+    """Rows around the widths at which a row no longer stays in the registers of its threads."""
+    for residual in (False, True):
+        rng = np.random.default_rng(29)
+        check(hip_backend_session, *cases.norm_case(3, width, residual, rng), cases.norm_bounds)
+        check(hip_backend_session, *cases.norm_grad_case(3, width, residual, rng), cases.norm_grad_bounds)

@@ -6,9 +6,45 @@ import pytest
 
 import host_kernel
 import operator_cases as cases
-from descent_amd import hip_backend
-from descent_amd.operators import OperatorKernel, OperatorSpec
+from descent_amd import Environment, hip_backend
+from descent_amd.operators import OperatorKernel, OperatorSpec, emit
 from descent_amd.shape import Shape
+from oracle.cpu_backend import CpuBackend
+
+
+def _grid(kernel):
+    """Workgroups of a kernel's launch, from the listing of a schedule that holds nothing else."""
+    env = Environment(CpuBackend())
+    operands = [env.static_parameter(list(v.output_shape), "p") for v in kernel.inputs]
+    results = [env.static_parameter(list(kernel.result_shapes()[i]), "r") for i in kernel.results]
+
+    def build(s):
+        got = emit([s.parameter_value(p) for p in operands], kernel.spec, len(results))
+        for p, a in zip(results, got):
+            s.write_parameter_value(p, a)
+
+    (grid,) = re.findall(r" grid (\d+)x", hip_backend.check_schedule(env.build_graph(build), fused=False))
+    return int(grid)
+
+
+def _kernels():
+    rng = np.random.default_rng(3)
+    out = []
+    for c in [(1, 1, False), (7, 100, True), (33, 2048, True), (600, 33, False), (2, 40000, True)]:
+        out += [cases.norm_case(*c, rng), cases.norm_grad_case(*c, rng)]
+    out += [cases.rotary_case(*c, rng) for c in cases.ROTARIES[:6]]
+    out += [cases.dual_case(*c, rng) for c in cases.DUALS if c[1] < 300]
+    # (batch, tokens, keys, heads, groups, dim, window, sinks, places)
+    for c in [(2, 1, 40, 4, 2, 16, 0, 0, "both"), (1, 3, 90, 2, 1, 30, 17, 4, "start"), (1, 33, 33, 1, 1, 256, 0, 0, "none"), (1, 70, 100, 3, 1, 48, 20, 5, "length"),
+              (2, 65, 65, 2, 2, 112, 9, 70, "length"), (1, 66, 130, 2, 1, 200, 64, 1, "both")]:
+        out += [cases.attention_case(*c, rng)] + cases.attention_grad_cases(*c, rng, pieces=3 if c[6] and c[7] else 0)
+        out += [cases.attention_case(*c, rng, splits=3)] if c[1] < 17 else []
+    return out
+
+
+def test_operators_stay_inside_their_operands():
+    for kernel, arrays in _kernels():
+        host_kernel.run(kernel, arrays, _grid(kernel))
 
 
 def _split_grid(kernel):
