@@ -397,6 +397,14 @@ class Array:
         return Array(s.ops.new_node(s.colour, shape, Op("WindowsToImage", tuple(stride_wh)), [self.node_id]), s)
 
     # -- sequence-model operators (kernels of their own; see operators.py) ---------------
+    def _lift_places(self, value) -> Optional["Array"]:
+        """Positions, starts and lengths: u32 arrays, or whole numbers that stand for an array of one."""
+        if value is None or isinstance(value, (Array, DualArray, Parameter)):
+            return None if value is None else self._lift(value)
+        if isinstance(value, bool) or not isinstance(value, (int, np.integer)) or not 0 <= value < 1 << 32:
+            raise ValueError(f"positions, starts and lengths are u32 arrays or a whole number of 32 bits, got {value!r}")
+        return self.scope.literal_u32(int(value))
+
     def _rows(self) -> "Array":
         n = self.shape[-1]
         return self.reshape([self.shape.element_count() // n, n])
@@ -421,10 +429,10 @@ class Array:
 
         layout     "half": pair i is (i, i + pairs); "interleaved": (2 i, 2 i + 1)
         positions  u32 array: [batch], the position of each sequence's first token (the others follow), or
-                   [batch, tokens]; None counts from 0
+                   [batch, tokens], or a whole number for a batch of one; None counts from 0
         inverse    turns back (the gradient of the rotation, with the same magnitude)"""
         frequencies = self._lift(frequencies)
-        positions = None if positions is None else self._lift(positions)
+        positions = self._lift_places(positions)
         spec = rotary_spec(self.shape, frequencies.shape, None if positions is None else positions.shape, layout, magnitude, inverse)
         return emit([self, frequencies] + ([] if positions is None else [positions]), spec, 1)[0]
 
@@ -448,17 +456,17 @@ class Array:
 
         Token t of sequence b stands at position start[b] + t and sees key j when j <= position, j < length[b] and,
         with a window, j > position - window or j < sinks.  A token at or past length[b] is padding: it sees nothing,
-        and a token that sees nothing gets zeros.  `start` and `length` are u32 arrays [batch]; without them the
-        queries are the last tokens of the keys, and every key counts.  `scale` defaults to dim^-0.5."""
+        and a token that sees nothing gets zeros.  `start` and `length` are u32 arrays [batch], or whole numbers
+        for a batch of one; without them the queries are the last tokens of the keys, and every key counts.  `scale` defaults to dim^-0.5."""
         k, v = self._lift(k), self._lift(v)
-        start, length = (None if a is None else self._lift(a) for a in (start, length))
+        start, length = self._lift_places(start), self._lift_places(length)
         return self._attention(k, v, window, sinks, scale, start, length)[0]
 
     def cache_append(self, rows, start) -> "Array":
         """self, [batch, capacity, width], with rows [batch, tokens, width] in place of its rows from start[b] on (u32
-        [batch]); rows past the capacity are dropped.  The buffer is updated in place, as by scatter_add: nothing else
+        [batch], or a whole number for a batch of one); rows past the capacity are dropped.  The buffer is updated in place, as by scatter_add: nothing else
         may read the old values."""
-        rows, start = self._lift(rows), self._lift(start)
+        rows, start = self._lift(rows), self._lift_places(start)
         return emit([self, rows, start], append_spec(self.shape, rows.shape, start.shape), 1)[0]
 
     def gated_dense(self, w_gate, w_up, activation: str = "silu") -> "Array":
@@ -762,7 +770,7 @@ class DualArray:
         q, dq = self.into_inner()
         k, dk = self._lift(k).into_inner()
         v, dv = self._lift(v).into_inner()
-        start, length = (None if a is None else q._lift(a) for a in (start, length))
+        start, length = q._lift_places(start), q._lift_places(length)
         out, lse, ints, scale = q._attention(k, v, window, sinks, scale, start, length)
         out, dout = out.with_empty_grad()
         places = [a for a in (start, length) if a is not None]

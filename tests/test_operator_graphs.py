@@ -58,3 +58,40 @@ def test_a_norm_that_no_loss_takes_beside_one_that_does():
     want, share = ref.rms_norm_grad(total, rho, d["w"], d["dy"], None)
     assert np.allclose(env.read_parameter(out["x"]), want, atol=1e-5) and np.array_equal(env.read_parameter(out["x"]), env.read_parameter(out["r"]))
     assert np.allclose(env.read_parameter(out["w"]), share.sum(0), atol=1e-5)
+
+
+def test_places_given_as_numbers():
+    """A start, a length or a position may be a number where an array of one would do: it is a whole number then, not the
+    bits of a float."""
+    env = Environment(CpuBackend())
+    rng = np.random.default_rng(3)
+    q, k, rows = rng.standard_normal((1, 2, 4, 6)), rng.standard_normal((1, 9, 2, 6)), rng.standard_normal((1, 2, 5))
+    p = {n: env.static_parameter_with_data(a.shape, n, a) for n, a in (("q", q), ("k", k), ("rows", rows), ("f", np.array([1.0, 0.1])))}
+    place = env.static_parameter([1], "place")
+    env.write_parameter(place, np.array([3], np.uint32))
+    results = []
+    for given in (None, 3, np.int64(3), np.uint32(3)):
+        out = [env.static_parameter(s, "out") for s in ([1, 2, 4, 6], [1, 2, 4, 6], [1, 2, 4, 6], [1, 9, 5])]
+        cache = env.static_parameter_with_data([1, 9, 5], "cache", np.zeros((1, 9, 5)))
+
+        def build(s):
+            at = s.parameter_value(place).to_u32_bits() if given is None else given
+            a, b = s.parameter_value(p["q"]), s.parameter_value(p["k"])
+            s.write_parameter_value(out[0], a.attention(b, b, start=at, length=at))
+            s.write_parameter_value(out[1], s.parameter(p["q"]).attention(s.parameter(p["k"]), s.parameter(p["k"]), start=at).value())
+            s.write_parameter_value(out[2], a.rotary(p["f"], at))
+            s.write_parameter_value(cache, s.parameter_value(cache).cache_append(p["rows"], at))
+
+        graph = env.build_graph(build)
+        hip_backend.check_schedule(graph)
+        env.run(graph, 0)
+        results.append([env.read_parameter(o) for o in out[:3]] + [env.read_parameter(cache)])
+    assert np.abs(results[0][1]).min() > 0 and not results[0][0].any()  # (a length of 3: both tokens are padding)
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert np.array_equal(a, b)
+    for bad in (3.0, -1, 1 << 32, True):
+        with pytest.raises(ValueError, match="whole number"):
+            env.build_graph(lambda s: s.parameter_value(p["q"]).attention(p["k"], p["k"], start=bad))
+        with pytest.raises(ValueError, match="whole number"):
+            env.build_graph(lambda s: s.parameter_value(p["q"]).rotary(p["f"], bad))
