@@ -456,16 +456,17 @@ class Array:
 
         Token t of sequence b stands at position start[b] + t and sees key j when j <= position, j < length[b] and,
         with a window, j > position - window or j < sinks.  A token at or past length[b] is padding: it sees nothing,
-        and a token that sees nothing gets zeros.  `start` and `length` are u32 arrays [batch], or whole numbers
-        for a batch of one; without them the queries are the last tokens of the keys, and every key counts.  `scale` defaults to dim^-0.5."""
+        and a token that sees nothing gets zeros.  `start` and `length` are u32 arrays [batch], or whole numbers for a
+        batch of one; without them the queries are the last tokens of the keys, and every key counts.  `scale` defaults
+        to dim^-0.5."""
         k, v = self._lift(k), self._lift(v)
         start, length = self._lift_places(start), self._lift_places(length)
         return self._attention(k, v, window, sinks, scale, start, length)[0]
 
     def cache_append(self, rows, start) -> "Array":
         """self, [batch, capacity, width], with rows [batch, tokens, width] in place of its rows from start[b] on (u32
-        [batch], or a whole number for a batch of one); rows past the capacity are dropped.  The buffer is updated in place, as by scatter_add: nothing else
-        may read the old values."""
+        [batch], or a whole number for a batch of one); rows past the capacity are dropped.  The buffer is updated in
+        place, as by scatter_add: nothing else may read the old values."""
         rows, start = self._lift(rows), self._lift_places(start)
         return emit([self, rows, start], append_spec(self.shape, rows.shape, start.shape), 1)[0]
 

@@ -296,7 +296,9 @@ string gen_rms_norm(const FusedKernel& fk, Generated* g) {
     for (int i : wide) quads = quads && Operand(d.inputs[i]).quads(d.inputs[i], 1);
     const int vec = quads ? 4 : 1;
     // a thread holds at most 16 elements of a row (8 in the gradient, which keeps four arrays of them) as long as
-    // 1024 threads suffice
+    // 1024 threads suffice.  Up to 32 it still keeps them: 2048 x 16384 (33.6 M elements, with a residual) takes 98 us
+    // forward and 124 back, 1024 x 32768 104 and 209 (the gradient spills 136 registers), and 512 x 65536 in two passes
+    // 143 and 172.
     const int64_t most = grad ? 8 : 16;
     int tpr = 64;
     while (tpr < 1024 && up(n, (int64_t)tpr * vec) * vec > most) tpr *= 2;
@@ -565,7 +567,7 @@ string gen_dual_matmul(const FusedKernel& fk, Generated* g) {
     // the smallest where even that many do not fill the CUs (1001 x 1366 columns x 512 k of both products: 32 us with
     // 128x128, 37 with 64x64; 1001 x 500, k 2 x 1366, not split: 113 and 98).  Up to 64 rows there are too few tiles for the
     // CUs and a step's latency counts: four groups of waves share k (16 x 4096 into 8000: 162 us with one group, 120 with
-    // two, 86 with four; 64 x 2048 into 1366: 83, 62, 46, and 66 with tiles of 64x64).
+    // two, 84 to 89 with four; 64 x 2048 into 1366: 83, 62, 47, and 66 with tiles of 64x64).
     struct Tile {
         int bm, bn, wm, wn, ahead, groups;
     };

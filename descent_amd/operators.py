@@ -247,8 +247,8 @@ def append_spec(cache: Shape, rows: Shape, start: Shape) -> OperatorSpec:
 
 def attention_splits(q: Shape, k: Shape, window, sinks: int) -> int:
     """Pieces that the keys of a call with few query rows are cut into.  A workgroup takes 16 rows (the queries of one
-    sequence and key head, those of the group's heads side by side) and walks its keys in steps of 64; with fewer than
-    512 workgroups -- two per CU -- the keys are split until there are as many, at 256 keys a piece or more."""
+    sequence and key head, those of the group's heads side by side) and deals its keys in blocks of 16 to its four waves;
+    with fewer than 512 workgroups -- two per CU -- the keys are split until there are as many, at 256 keys a piece or more."""
     batch, tokens, heads, _ = q
     groups = k[2]
     rows = tokens * (heads // groups)

@@ -176,8 +176,10 @@ typedef struct dsc_pe_op {
  *   ATTENTION_GRAD_KEY_VALUE  in  q, k, v, d out (all s), log denominators, that sum, (those two), (start), (length)
  *                  op_int {window, sinks, as above, pieces or 0: the two are not given and nothing is left out}
  *                  out 0: dk; 1: dv
- *                  (attention: what a row does not see takes no part, whatever it holds; an element that it sees and that
- *                  is not finite makes its results NaN, or infinite in the calls for few rows)
+ *                  (attention: what a row does not see takes no part, whatever it holds.  A query that is not finite makes
+ *                  its row and the row's denominator NaN, a key or value that is NaN what it takes part in.  An infinite
+ *                  key or value gives what 32-bit arithmetic gives -- a score of -inf weighs nothing -- in calls of up to
+ *                  64 rows per key head, in pieces and for heads above 128, and NaN in the others.)
  *   CACHE_APPEND   in  rows [batch,tokens,width] (s), start [batch]     op_int {capacity}
  *                  out 0 (in/out, as SCATTER_ADD's accumulator): [batch,capacity,width]; row t of sequence b replaces the
  *                  cache's row start[b] + t, rows past the capacity are dropped
