@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import operator_cases as cases
-from descent_amd.operators import ACTIVATIONS, DUAL_BOTH, DUAL_GATED, DUAL_SUM, OperatorSpec
+from descent_amd.operators import ACTIVATIONS, DUAL_BOTH, DUAL_GATED, DUAL_SUM, OperatorKernel, OperatorSpec
 from descent_amd.shape import Shape, View
 from oracle import operators as ref
 from test_gpu_operators import check, launch
@@ -202,3 +202,65 @@ def test_wide_norms(hip_backend_session, width):
         rng = np.random.default_rng(29)
         check(hip_backend_session, *cases.norm_case(3, width, residual, rng), cases.norm_bounds)
         check(hip_backend_session, *cases.norm_grad_case(3, width, residual, rng), cases.norm_grad_bounds)
+
+
+@pytest.mark.parametrize("tokens,dim", [(1, 64), (70, 64), (70, 160)])
+def test_a_cache_of_more_than_2_31_elements(hip_backend_session, tokens, dim):
+    """The last keys of the last sequence lie past 2^31 elements: appended there, and seen through a window."""
+    be, rng = hip_backend_session, np.random.default_rng(30)
+    keys, window, tail = (1 << 30) // dim + 128, 40, 128
+    q, k, v = (cases.normal(rng, 2, n, 1, dim) for n in (tokens, tail, tail))
+    places = [np.full(2, keys - tokens, np.uint32), np.full(2, keys, np.uint32)]
+    cache = Shape((2, keys, 1, dim))
+    whole = []
+    for rows in (k, v):  # only the rows that are seen are ever written; the rest stays as allocated
+        h = be.alloc(cache.buffer_size())
+        whole.append(h)
+        handles = []
+        for a in cases.flat([rows.reshape(2, tail, dim), np.full(2, keys - tail, np.uint32)]):
+            handles.append(be.alloc(a.nbytes))
+            be.write(handles[-1], 0, a)
+        kernel = OperatorKernel(OperatorSpec("CacheAppend", (keys,)), (Shape((2, tail, dim)).identity_view(), Shape((2,)).identity_view()), (0,))
+        be.launch(kernel, handles + [h], 0)
+        last = np.frombuffer(be.read(h, cache.buffer_size() - 4 * tail * dim, 4 * tail * dim), np.float32)
+        assert np.array_equal(last, rows[1].ravel())
+        for a in handles:
+            be.free(a)
+    handles = []
+    for a in cases.flat([q] + places):
+        handles.append(be.alloc(a.nbytes))
+        be.write(handles[-1], 0, a)
+    views = (Shape(q.shape).identity_view(), cache.identity_view(), cache.identity_view()) + (Shape((2,)).identity_view(),) * 2
+    kernel = OperatorKernel(OperatorSpec("Attention", (window, 0, 3, 1), (dim ** -0.5,)), views, (0, 1))
+    out = [be.alloc(s.buffer_size()) for s in kernel.result_shapes()]
+    be.launch(kernel, [handles[0]] + whole + handles[1:] + out, 0)
+    got = [np.frombuffer(be.read(h, 0, s.buffer_size()), np.float32).reshape(tuple(s)) for h, s in zip(out, kernel.result_shapes())]
+    for h in handles + whole + out:
+        be.free(h)
+    arrays = [q, k, v, np.full(2, tail - tokens, np.uint32), np.full(2, tail, np.uint32)]
+    small = cases.kernel(kernel.spec, arrays)
+    want = ref.evaluate(small, cases.flat(arrays))
+    _agree(got, want, cases.attention_bounds(small, arrays, want))
+
+
+@pytest.mark.parametrize("dim", [48, 64, 136])
+def test_sinks_pieces_pass_what_is_not_a_number_on(hip_backend_session, dim):
+    """A NaN query past the window reaches the gradients of the sinks and of its window, a row of padding reaches nothing."""
+    case = (1, 200, 200, 4, 2, dim, 20, 5, "length")
+    (_, _), (whole, ka), (far, fa), (joined, ja) = cases.attention_grad_cases(*case, np.random.default_rng(31), 3)
+    clean = [a.copy() for a in ka]
+    bounds = cases.attention_grad_bounds(whole, clean, ref.evaluate(whole, cases.flat(clean)))
+    length = int(ka[-1][0])
+    assert 160 < length < 200
+    for arrays in (ka, fa, ja):
+        for i in (0, 4, 5):
+            arrays[i][0, 150, 1] = np.nan
+        for i in (0, 3):
+            arrays[i][0, length:] = np.nan
+    want = ref.evaluate(whole, cases.flat(ka))
+    assert np.isnan(want[0][0, :5, 0]).all() and np.isnan(want[0][0, 131:151, 0]).all() and np.isfinite(want[0][0, 5:131]).all()
+    pieces = launch(hip_backend_session, far, fa)
+    for p in pieces:
+        assert np.isnan(p.sum(0)[0, :, 0]).all() and np.isfinite(p[:, :, :, 1]).all()
+    got = launch(hip_backend_session, joined, ja[:6] + pieces + ja[8:])
+    _agree(got, want, [2 * b for b in bounds])
